@@ -124,6 +124,35 @@ int b200_rope_forward(b200_ctx *ctx, void *q, void *k, const float *cos_table, c
 int b200_rope_backward(b200_ctx *ctx, void *grad, const float *cos_table, const float *sin_table, size_t batch,
                        size_t heads, size_t seq_len, size_t head_dim, b200_dtype dtype);
 
+/* ---- RoPE at given positions, for batches whose tokens stand anywhere (ragged batches, long contexts).
+ * Interleaved pairs (2i, 2i+1) as above, or pairs (i, i + rotary_dim/2) of the half layout; only the first rotary_dim elements of
+ * each head turn (even, 0 .. head_dim), the rest is copied.  Pair i turns by position * freqs[i]. */
+enum { B200_ROPE_INTERLEAVED = 0, B200_ROPE_HALF = 1 };                                                        /* layout */
+enum { B200_ROPE_PLAIN = 0, B200_ROPE_LINEAR = 1, B200_ROPE_NTK = 2, B200_ROPE_YARN = 3, B200_ROPE_BANDS = 4 }; /* scaling */
+typedef struct {
+  size_t head_dim, rotary_dim;
+  int layout, scaling;
+  float base;                                 /* PLAIN: freqs[i] = base^(-2i/rotary_dim) */
+  float factor;                               /* LINEAR: freqs / factor; NTK: base * factor^(rotary_dim/(rotary_dim-2)) */
+  float original_len, beta_fast, beta_slow;   /* YARN: pairs that turn more than beta_fast times over original_len keep their frequency, those below beta_slow are divided by factor, a ramp between */
+  float low_freq_factor, high_freq_factor;    /* BANDS: the same by wavelength: below original_len/high_freq_factor kept, above original_len/low_freq_factor divided, a blend between */
+  float amplitude;                            /* multiplies the rotated elements; 0: 1, or 0.1 ln(factor) + 1 for YARN */
+} b200_rope_config;
+/* The amplitude in effect. */
+float b200_rope_amplitude(const b200_rope_config *cfg);
+/* Frequencies in radians per position, device fp64 [rotary_dim/2] (64 bits: at position 10^6 a 32-bit frequency is off by a
+ * visible angle).  Laid out once; base, factor, original_len and the betas matter only here. */
+int b200_rope_frequencies(b200_ctx *ctx, const b200_rope_config *cfg, double *freqs);
+/* q [tokens, q_heads, head_dim] and k [tokens, kv_heads, head_dim], row strides ld_* in elements; positions device int32 [tokens],
+ * any sign.  q or k may be NULL.  Outputs may be the inputs themselves (in place) but not overlap them otherwise. */
+int b200_rope_positions_forward(b200_ctx *ctx, const b200_rope_config *cfg, const double *freqs, const int32_t *positions, const void *q,
+                                void *q_out, size_t ld_q, size_t ld_q_out, size_t q_heads, const void *k, void *k_out, size_t ld_k,
+                                size_t ld_k_out, size_t kv_heads, size_t tokens, b200_dtype dtype);
+/* Gradients of the inputs from those of the outputs: the transposed rotation, same amplitude. */
+int b200_rope_positions_backward(b200_ctx *ctx, const b200_rope_config *cfg, const double *freqs, const int32_t *positions, const void *dq,
+                                 void *dq_out, size_t ld_dq, size_t ld_dq_out, size_t q_heads, const void *dk, void *dk_out, size_t ld_dk,
+                                 size_t ld_dk_out, size_t kv_heads, size_t tokens, b200_dtype dtype);
+
 /* ---- SwiGLU: metal_bridge::swiglu_forward / swiglu_backward (MetalBridge.hpp:65-67) */
 int b200_swiglu_forward(b200_ctx *ctx, const void *gate, const void *up, void *out, size_t n, b200_dtype dtype);
 int b200_swiglu_backward(b200_ctx *ctx, const void *grad_output, const void *gate, const void *up, void *grad_gate,
@@ -166,6 +195,41 @@ int b200_fused_attn_bwd(b200_ctx *ctx, const void *Q, const void *K, const void 
 int b200_flash_attn_bwd(b200_ctx *ctx, const void *Q, const void *K, const void *V, const void *O, const void *dO,
                         const float *lse, void *dQ, void *dK, void *dV, size_t batch, size_t n_heads, size_t n_kv,
                         size_t seq_len, size_t head_dim, b200_dtype dtype);
+
+/* ---- paged key/value cache: sequences of different lengths share one pool of pages.
+ * Position p of sequence s lives in page page_table[s * table_ld + p / page_size], slot p % page_size; element d of KV head h
+ * there is at page * page_stride + slot * token_stride + h * head_stride + d (elements), in k and in v alike.  Any page_size from 1 on.
+ * Sequences may share pages (a common prefix).  The tables and lengths are read on the device, so a captured step replays with
+ * new ones.  What they say is checked there: a page id outside [0, n_pages), a length beyond the table, or rows that q_start
+ * puts outside [0, rows) touch no memory outside the arrays; b200_sync then reports B200_ERR_INVALID, and the results of
+ * that sequence are unspecified. */
+typedef struct {
+  void *k, *v;                                             /* device */
+  size_t n_pages, page_size, n_kv, head_dim;
+  size_t page_stride, token_stride, head_stride;           /* elements; [n_pages, page_size, n_kv, head_dim]: page_size*n_kv*head_dim, n_kv*head_dim, head_dim */
+  b200_dtype dtype;
+} b200_paged_cache;
+/* Sequence s brings rows q_start[s] .. q_start[s+1]-1 of q / k / v, its newest tokens; kv_len[s] positions of the cache are
+ * valid once they are in it.  Row i of the sequence stands at position kv_len[s] - (its rows) + i; rows at negative positions are padding. */
+typedef struct {
+  const int32_t *q_start, *kv_len, *page_table;            /* device: [n_seq + 1], [n_seq], [n_seq, table_ld] */
+  size_t n_seq, table_ld;
+  size_t rows;                                             /* rows that q / k / v hold; those from q_start[n_seq] on are left alone */
+  size_t max_q;                                            /* no sequence brings more rows than this (0: rows) */
+} b200_paged_batch;
+/* Writes the new rows of k and v [rows, n_kv, head_dim] (row strides ld_k, ld_v) to their slots.  With `rope` the keys are rotated
+ * by their position on the way, and q [rows, q_heads, head_dim] (optional) is rotated into q_out (may be q); without it q is copied.
+ * No two rows may have the same slot. */
+int b200_paged_append(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, const void *k, const void *v, size_t ld_k,
+                      size_t ld_v, const b200_rope_config *rope, const double *freqs, const void *q, void *q_out, size_t ld_q,
+                      size_t ld_q_out, size_t q_heads);
+/* Causal attention of the new rows over the cache (which holds them already): o [rows, n_heads, head_dim] and, optional, lse fp32
+ * [rows, n_heads], the log-sum-exp of the scaled scores.  scale 0: 1/sqrt(head_dim).  Rows that see nothing get o = 0, lse = -inf.
+ * Positions from kv_len on are never used, whatever their slots hold.  head_dim up to 256.
+ * The workspace is the caller's: calls that may overlap, captured graphs among them, each need their own. */
+int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, size_t n_heads, size_t *bytes);
+int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, const void *q, size_t ld_q, void *o,
+                    size_t ld_o, float *lse, size_t n_heads, float scale, void *workspace, size_t workspace_bytes);
 
 /* ---- embedding gather: metal_bridge::embedding_forward (MetalBridge.hpp:86-88) */
 int b200_embedding_forward(b200_ctx *ctx, const uint32_t *token_ids, const void *table, void *output,
@@ -301,6 +365,18 @@ typedef struct {
 int b200_sample(b200_ctx *ctx, const void *logits, b200_dtype dtype, size_t batch, size_t vocab, int32_t *history,
                 size_t hist_len, size_t hist_ld, int append, const b200_sampler_config *cfg, uint64_t step,
                 int32_t *out_tokens, float *out_threshold, int32_t *out_kept);
+/* One sampling step from given random numbers, with settings per row: device arrays of `batch` values, each optional but uniform.
+ * logits [batch, vocab] with row stride ld.  Ids are ordered by logit, equal logits by id (lowest first); -inf and NaN logits are
+ * masked ids.  With w_i = exp((l_i - max l) / temperature), in 64 bits:
+ *   temperature <= 0 or NaN: the first id (the others are not looked at);
+ *   top_k in 1 .. vocab-1: the first top_k ids stay;    top_p < 1: of these, an id stays while the weight before it is below
+ *   top_p x their weight (the first always);            min_p > 0: ids with w_i < min(min_p, 1) go.
+ * The token is the lowest id that stays whose cumulative weight, in id order, exceeds uniform x the weight of all that stay; uniform is
+ * taken into [0, 1).  out_kept (optional): how many ids stay; out_prob (optional): the token's share of their weight.
+ * A row with nothing to draw from gets token -1.  The same inputs always give the same outputs; nothing is allocated. */
+int b200_sample_given(b200_ctx *ctx, const void *logits, b200_dtype dtype, size_t batch, size_t vocab, size_t ld, const float *temperature,
+                      const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform, int32_t *out_tokens,
+                      int32_t *out_kept, float *out_prob);
 /* Allocates K/V caches for `batch` sequences of up to max_total_len positions (<= max_seq_len of the model).  A later
  * call that asks for more sequences or positions re-allocates (the cached keys/values of the earlier generation are
  * dropped); a call that fits the existing caches keeps them. */

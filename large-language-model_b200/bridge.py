@@ -52,6 +52,54 @@ class SamplerConfig(C.Structure):
         return cls(temperature, top_p, repetition_penalty, top_k, seed, min(len(whitespace_ids), 8), (_i * 8)(*ws))
 
 
+class RopeConfig(C.Structure):
+    """Rotary embedding at given positions: layout, rotated part of the head, scaling for long contexts."""
+    _fields_ = [("head_dim", _sz), ("rotary_dim", _sz), ("layout", _i), ("scaling", _i)] + [
+        (n, _f) for n in ("base", "factor", "original_len", "beta_fast", "beta_slow", "low_freq_factor", "high_freq_factor", "amplitude")]
+    LAYOUTS = ("interleaved", "half")
+    SCALINGS = ("plain", "linear", "ntk", "yarn", "bands")
+
+    @classmethod
+    def make(cls, head_dim, rotary_dim=None, layout="interleaved", scaling="plain", base=10000.0, factor=1.0, original_len=2048.0,
+             beta_fast=32.0, beta_slow=1.0, low_freq_factor=1.0, high_freq_factor=4.0, amplitude=0.0):
+        return cls(head_dim, head_dim if rotary_dim is None else rotary_dim, cls.LAYOUTS.index(layout), cls.SCALINGS.index(scaling), base,
+                   factor, original_len, beta_fast, beta_slow, low_freq_factor, high_freq_factor, amplitude)
+
+
+class _PagedCache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp)] + [(n, _sz) for n in ("n_pages", "page_size", "n_kv", "head_dim", "page_stride", "token_stride",
+                                                             "head_stride")] + [("dtype", _i)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q_start", "kv_len", "page_table")] + [(n, _sz) for n in ("n_seq", "table_ld", "rows", "max_q")]
+
+
+class PagedCache:
+    """Pages of keys and values: two device arrays [n_pages, page_size, n_kv, head_dim], or any strides (in elements)."""
+
+    def __init__(self, k, v, page_stride=None, token_stride=None, head_stride=None):
+        n, p, h, d = k.shape
+        if tuple(v.shape) != (n, p, h, d) or v.dtype != k.dtype:
+            raise B200Error("k and v pages must be alike")
+        self.k, self.v = k, v
+        self.struct = _PagedCache(k.ptr, v.ptr, n, p, h, d, p * h * d if page_stride is None else page_stride,
+                                  h * d if token_stride is None else token_stride, d if head_stride is None else head_stride, k.code)
+        self.ref = C.byref(self.struct)
+
+
+class PagedBatch:
+    """A ragged batch of new tokens over a paged cache; int32 device arrays q_start [n_seq + 1], kv_len [n_seq], page_table [n_seq, m]."""
+
+    def __init__(self, q_start, kv_len, page_table, rows: int, max_q: int = 0):
+        n, m = page_table.shape
+        if kv_len.size != n or q_start.size != n + 1:
+            raise B200Error("q_start, kv_len and page_table must agree on the number of sequences")
+        self.arrays = (q_start, kv_len, page_table)
+        self.struct = _PagedBatch(q_start.ptr, kv_len.ptr, page_table.ptr, n, m, rows, max_q)
+        self.ref = C.byref(self.struct)
+
+
 class AdamWParams(C.Structure):
     _fields_ = [(n, _f) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "bias_correction1",
                                   "bias_correction2")]
@@ -86,6 +134,10 @@ _SIGS = {
     "b200_rope_tables": (_i, [_vp, _vp, _vp, _sz, _sz, _f]),
     "b200_rope_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i]),
     "b200_rope_backward": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _i]),
+    "b200_rope_amplitude": (_f, [_vp]),
+    "b200_rope_frequencies": (_i, [_vp, _vp, _vp]),
+    "b200_rope_positions_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _i]),
+    "b200_rope_positions_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _i]),
     "b200_swiglu_forward": (_i, [_vp, _vp, _vp, _vp, _sz, _i]),
     "b200_swiglu_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i]),
     "b200_fused_swiglu_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _i]),
@@ -96,6 +148,9 @@ _SIGS = {
     "b200_flash_attn_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i]),
     "b200_fused_attn_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i]),
     "b200_flash_attn_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i]),
+    "b200_paged_append": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz]),
+    "b200_paged_attn_workspace": (_i, [_vp, _vp, _vp, _sz, C.POINTER(_sz)]),
+    "b200_paged_attn": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _f, _vp, _sz]),
     "b200_embedding_forward": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _i]),
     "b200_embedding_backward": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _i]),
     "b200_cross_entropy": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _i]),
@@ -133,6 +188,7 @@ _SIGS = {
     "b200_model_layer_forward": (_i, [_vp, _sz, _vp, _vp, _sz, _sz]),
     "b200_model_layer_backward": (_i, [_vp, _sz, _vp, _vp, _sz, _sz]),
     "b200_sample": (_i, [_vp, _vp, _i, _sz, _sz, _vp, _sz, _sz, _i, C.POINTER(SamplerConfig), C.c_uint64, _vp, _vp, _vp]),
+    "b200_sample_given": (_i, [_vp, _vp, _i, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_model_decode_begin": (_i, [_vp, _sz, _sz]),
     "b200_model_prefill": (_i, [_vp, _vp, _sz, _sz, _vp]),
     "b200_model_decode_step": (_i, [_vp, _vp, _sz, _sz, _vp]),
@@ -171,11 +227,12 @@ def _np_ptr(a: np.ndarray):
 
 
 class DeviceArray:
-    """A device allocation with shape and element type ("f32", "bf16", "i32", "u32")."""
+    """A device allocation with shape and element type ("f32", "bf16", "i32", "u32", "f64")."""
+    owned = True
 
     def __init__(self, ctx: "Context", shape, dtype: str):
         self.ctx, self.shape, self.dtype = ctx, tuple(int(s) for s in np.atleast_1d(shape)), dtype
-        self.itemsize = 2 if dtype == "bf16" else 4
+        self.itemsize = {"bf16": 2, "f64": 8}.get(dtype, 4)
         self.size = int(np.prod(self.shape)) if len(self.shape) else 1
         self.nbytes = self.size * self.itemsize
         p = _vp()
@@ -197,6 +254,8 @@ class DeviceArray:
             host = np.ascontiguousarray(a, np.float32)
         elif self.dtype == "i32":
             host = np.ascontiguousarray(a, np.int32)
+        elif self.dtype == "f64":
+            host = np.ascontiguousarray(a, np.float64)
         else:
             host = np.ascontiguousarray(a, np.uint32)
         assert host.size == self.size, (host.size, self.size)
@@ -205,7 +264,7 @@ class DeviceArray:
         return self
 
     def download(self) -> np.ndarray:
-        npdt = {"bf16": np.uint16, "f32": np.float32, "i32": np.int32, "u32": np.uint32}[self.dtype]
+        npdt = {"bf16": np.uint16, "f32": np.float32, "i32": np.int32, "u32": np.uint32, "f64": np.float64}[self.dtype]
         host = np.empty(self.shape, npdt)
         self.ctx._check(self.ctx.lib.b200_memcpy_d2h(self.ctx.h, _np_ptr(host), self.ptr, self.nbytes))
         self.ctx.sync()
@@ -216,9 +275,20 @@ class DeviceArray:
         return self
 
     def free(self):
-        if self.ptr:
+        if self.ptr and self.owned:
             self.ctx.lib.b200_free(self.ctx.h, self.ptr)
             self.ptr = None
+
+
+class DeviceView(DeviceArray):
+    """Device memory that belongs to someone else (another library's tensor), seen as a device array."""
+    owned = False
+
+    def __init__(self, ctx: "Context", ptr: int, shape, dtype: str):
+        self.ctx, self.shape, self.dtype = ctx, tuple(int(s) for s in shape), dtype
+        self.itemsize = {"bf16": 2, "f64": 8}.get(dtype, 4)
+        self.size = int(np.prod(self.shape)) if len(self.shape) else 1
+        self.nbytes, self.ptr = self.size * self.itemsize, ptr
 
 
 class Context:
@@ -256,6 +326,17 @@ class Context:
 
     def stream_ptr(self) -> int:
         return self.lib.b200_stream(self.h) or 0
+
+    def use_stream(self, handle: int):
+        """Enqueue on another library's stream from here on; 0 is the legacy default stream (the context's own: `own_stream`)."""
+        self._check(self.lib.b200_set_stream(self.h, handle or 1))      # 1: cudaStreamLegacy
+
+    def own_stream(self):
+        self._check(self.lib.b200_set_stream(self.h, None))
+
+    def wrap(self, ptr: int, shape, dtype="f32") -> DeviceView:
+        """Another library's device memory as a device array; it must outlive the work enqueued on it."""
+        return DeviceView(self, ptr, shape, dtype)
 
     def launch_count(self) -> int:
         return int(self.lib.b200_launch_count(self.h))
@@ -325,6 +406,33 @@ class Context:
         B, h, S, hd = g.shape
         self._check(self.lib.b200_rope_backward(self.h, g.ptr, cos.ptr, sin.ptr, B, h, S, hd, g.code))
 
+    def rope_frequencies(self, cfg: "RopeConfig"):
+        f = self.empty((max(1, cfg.rotary_dim // 2),), "f64")
+        self._check(self.lib.b200_rope_frequencies(self.h, C.byref(cfg), f.ptr))
+        return f
+
+    def _rope_positions(self, fn, cfg, freqs, positions, q, k, out):
+        if out is None:
+            out = (self.empty(q.shape, q.dtype) if q is not None else None, self.empty(k.shape, k.dtype) if k is not None else None)
+        a, (qo, ko) = q if q is not None else k, out
+        hd = a.shape[2]
+        if hd != cfg.head_dim or positions.size != a.shape[0] or (q is not None and k is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0] or k.shape[2] != hd)):
+            raise B200Error("rope_positions: q [tokens, heads, head_dim], k and positions must agree")
+        for x, y in ((q, qo), (k, ko)):
+            if x is not None and (y is None or y.shape != x.shape or y.dtype != x.dtype):
+                raise B200Error("rope_positions: outputs must be like the inputs")
+        nq, nk = q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0
+        self._check(fn(self.h, C.byref(cfg), freqs.ptr if freqs is not None else None, positions.ptr, q.ptr if nq else None, qo.ptr if nq else None,
+                       nq * hd, nq * hd, nq, k.ptr if nk else None, ko.ptr if nk else None, nk * hd, nk * hd, nk, a.shape[0], a.code))
+        return out
+
+    def rope_positions_forward(self, cfg, freqs, positions, q, k=None, out=None):
+        """Rotates q and k [tokens, heads, head_dim] by each token's position; out=(q, k) works in place."""
+        return self._rope_positions(self.lib.b200_rope_positions_forward, cfg, freqs, positions, q, k, out)
+
+    def rope_positions_backward(self, cfg, freqs, positions, dq, dk=None, out=None):
+        return self._rope_positions(self.lib.b200_rope_positions_backward, cfg, freqs, positions, dq, dk, out)
+
     def swiglu_forward(self, gate, up):
         out = self.empty(gate.shape, gate.dtype)
         self._check(self.lib.b200_swiglu_forward(self.h, gate.ptr, up.ptr, out.ptr, gate.size, gate.code))
@@ -377,6 +485,44 @@ class Context:
         self._check(self.lib.b200_flash_attn_bwd(self.h, q.ptr, k.ptr, v.ptr, o.ptr, dO.ptr, lse.ptr, dq.ptr, dk.ptr, dv.ptr,
                                                  B, nH, k.shape[1], S, hd, q.code))
         return dq, dk, dv
+
+    def paged_append(self, cache: "PagedCache", batch: "PagedBatch", k, v, rope=None, freqs=None, q=None, q_out=None):
+        """Writes new keys and values [rows, n_kv, head_dim] to the cache; with `rope` k (and q, into q_out) is rotated on the way."""
+        (rows, n, hd), st = k.shape, cache.struct
+        if (v.shape != k.shape or v.dtype != k.dtype or k.dtype != cache.k.dtype or rows != batch.struct.rows or n != st.n_kv or hd != st.head_dim or
+                (q is not None and (q.shape[0] != rows or q.shape[2] != hd or q.dtype != k.dtype))):
+            raise B200Error("paged_append: k, v and q must match the cache and the batch")
+        if q is not None and q_out is None:
+            q_out = self.empty(q.shape, q.dtype)
+        elif q is not None and (q_out.shape != q.shape or q_out.dtype != q.dtype):
+            raise B200Error("paged_append: q_out must be like q")
+        nh = q.shape[1] if q is not None else 0
+        self._check(self.lib.b200_paged_append(self.h, cache.ref, batch.ref, k.ptr, v.ptr, n * hd, n * hd, C.byref(rope) if rope is not None else None,
+                                               freqs.ptr if freqs is not None else None, q.ptr if nh else None, q_out.ptr if nh else None, nh * hd, nh * hd, nh))
+        return q_out
+
+    def paged_attn_workspace(self, cache, batch, n_heads: int) -> int:
+        n = _sz(0)
+        self._check(self.lib.b200_paged_attn_workspace(self.h, cache.ref, batch.ref, n_heads, C.byref(n)))
+        return int(n.value)
+
+    def paged_attn(self, cache: "PagedCache", batch: "PagedBatch", q, out=None, lse=None, scale=0.0, workspace=None):
+        """Causal attention of q [rows, n_heads, head_dim] over the paged cache.  Without `workspace` one is allocated for this call."""
+        (rows, nh, hd), st = q.shape, cache.struct
+        if rows != batch.struct.rows or hd != st.head_dim or q.dtype != cache.k.dtype:
+            raise B200Error("paged_attn: q must match the cache and the batch")
+        out = self.empty(q.shape, q.dtype).zero() if out is None else out
+        if out.shape != q.shape or out.dtype != q.dtype or (lse is not None and (lse.size != rows * nh or lse.dtype != "f32")):
+            raise B200Error("paged_attn: out must be like q, lse f32 [rows, n_heads]")
+        own = workspace is None
+        if own:
+            workspace = self.empty((self.paged_attn_workspace(cache, batch, nh) // 4,))
+        self._check(self.lib.b200_paged_attn(self.h, cache.ref, batch.ref, q.ptr, nh * hd, out.ptr, nh * hd, lse.ptr if lse is not None else None, nh,
+                                             scale, workspace.ptr, workspace.nbytes))
+        if own:
+            self._live.remove(workspace)
+            workspace.free()
+        return out
 
     def embedding_forward(self, ids, table):
         V, H = table.shape
@@ -434,6 +580,17 @@ class Context:
                                          hist_len, history.shape[1] if history is not None else 0, int(append),
                                          C.byref(sampler), step, tok.ptr, thr.ptr, kept.ptr))
         return tok, thr, kept
+
+    def sample_given(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+        """One sampling step from given random numbers with settings per row (device arrays [batch]); returns (tokens, kept, prob)."""
+        B, V = logits.shape
+        tok, kept, prob = out if out is not None else (self.empty((B,), "i32"), self.empty((B,), "i32"), self.empty((B,), "f32"))
+        for x, t in ((uniform, "f32"), (temperature, "f32"), (top_k, "i32"), (top_p, "f32"), (min_p, "f32"), (tok, "i32"), (kept, "i32"), (prob, "f32")):
+            if x is not None and (x.size != B or x.dtype != t):
+                raise B200Error("sample_given: settings and outputs hold one value a row")
+        p = [x.ptr if x is not None else None for x in (temperature, top_k, top_p, min_p, uniform, tok, kept, prob)]
+        self._check(self.lib.b200_sample_given(self.h, logits.ptr, logits.code, B, V, V, *p))
+        return tok, kept, prob
 
     def adamw_step(self, p, g, m, v, lr, beta1, beta2, eps, wd, step, shadow=None):
         bc1 = float(np.float32(1.0) - np.float32(beta1) ** np.float32(step))

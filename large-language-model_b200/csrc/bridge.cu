@@ -122,6 +122,7 @@ extern "C" int b200_sync(b200_ctx *ctx) {
   if (st != 0) {
     cudaMemsetAsync(ctx->dev_status, 0, sizeof(int), ctx->stream);
     if (st == 2) return b200_fail(ctx, B200_ERR_INVALID, "token id out of range in embedding lookup");
+    if (st == 3) return b200_fail(ctx, B200_ERR_INVALID, "paged batch: a page id, a length or a row range is out of range");
     return b200_fail(ctx, B200_ERR_DEVICE_WAIT, "a device-side wait gave up (code %d)", st);
   }
   return B200_OK;

@@ -1,0 +1,331 @@
+// Attention of a ragged batch of new tokens over a paged key/value cache: entry point, the CUDA-core kernel that takes
+// every type, head size and alignment, and the join of partial results.
+//
+//   o = sum_j softmax_j(scale q . k_j) v_j over the keys 0 .. p of the row's own sequence, p the row's position;
+//   lse = log sum_j exp(scale q . k_j).  Rows that see no key get o = 0 and lse = -inf.
+// The single-token and the causal attention of cpp/src/Attention.cpp:236-280, with keys found through a page table.
+//
+// The CUDA-core kernel: blocks of 32 rows (token, query head of the group) x tiles of 32 keys, one pass with a running
+// maximum and sum.  Warp w owns rows w, w + 4, ...; in the scores a lane is a key, in the product with V four dimensions.
+// Keys and values pass through shared memory in 32 bits.  Bound by shared-memory reads (12 per 32 multiply-adds of a warp
+// with all its rows, fewer instructions with few rows).
+#include "paged_attn.cuh"
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+namespace {
+
+constexpr int THREADS = 128, ROWS = 32, TILE = 32, WROWS = ROWS / 4;
+
+// HJ: 128-dimension slices of the head.
+template <class T, int HJ>
+__global__ void __launch_bounds__(THREADS)
+paged_attn_simt_kernel(PagedAttnArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ __align__(16) float smem[];
+  __shared__ long long red[33];
+  __shared__ paged::Place place;
+  __shared__ int page_s[TILE];
+  const int hd = a.b.hd, hd4 = (hd + 3) & ~3, kst = hd4 + 4, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float *sK = smem, *sV = sK + TILE * kst, *sQ = sV + TILE * hd4, *sP = sQ + ROWS * hd4 + warp * WROWS * TILE;
+  const long long total = paged::line_total<THREADS>(a.b, a.plan, red);
+  const int n = paged::line_ctas(total, a.n_cta, a.min_units), c = blockIdx.x;
+  if (c >= n || total == 0) return;
+  long long u = paged::line_at(total, n, c);
+  const long long end = paged::line_at(total, n, c + 1);
+  paged::line_find<THREADS>(a.b, a.plan, u, red, &place);
+  paged::Place pl = place;
+  const float sl2 = a.scale * PAGED_LOG2E;
+  while (u < end) {
+    const int tiles = a.plan.tiles(pl.q, pl.block), kt1 = (int)min((long long)tiles, pl.kt + (end - u));
+    // ---- queries of the block, rows that do not exist as zeros
+    __syncthreads();
+    for (int i = tid; i < ROWS * hd4; i += THREADS) {
+      const int r = i / hd4, d = i - r * hd4;
+      int row, head, pos;
+      float x = 0.f;
+      if (paged_row(a, pl, r, row, head, pos) && d < hd) x = to_f(((const T *)a.q)[(size_t)row * a.ld_q + (size_t)head * hd + d]);
+      sQ[i] = x;
+    }
+    int limit[WROWS], out_row[WROWS], out_head[WROWS], live = 0;      // limit: keys the row sees
+    float m[WROWS], l[WROWS];
+    float4 acc[WROWS][HJ];
+#pragma unroll
+    for (int i = 0; i < WROWS; ++i) {
+      int pos = 0;
+      const bool has = paged_row(a, pl, warp + 4 * i, out_row[i], out_head[i], pos);
+      limit[i] = has ? min(max(pos + 1, 0), pl.q.len) : 0;
+      if (has) live = i + 1;
+      m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < HJ; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int kt = pl.kt; kt < kt1; ++kt) {
+      __syncthreads();
+      if (tid < TILE) {
+        const int pos = kt * TILE + tid;
+        page_s[tid] = pos < pl.q.len ? paged::page_of(a.b, pl.seq, pos) : -1;
+      }
+      __syncthreads();
+      for (int i = tid; i < TILE * hd4; i += THREADS) {
+        const int r = i / hd4, d = i - r * hd4, page = page_s[r];
+        float x = 0.f, y = 0.f;                                        // positions never written may hold anything: read as zero
+        if (page >= 0 && d < hd) {
+          const long long at = (long long)page * a.b.page_stride + (long long)((kt * TILE + r) % a.b.page_size) * a.b.token_stride + (long long)pl.kvh * a.b.head_stride + d;
+          x = to_f(((const T *)a.k)[at]); y = to_f(((const T *)a.v)[at]);
+        }
+        sK[r * kst + d] = x; sV[i] = y;
+      }
+      __syncthreads();
+      if (live == 0) continue;
+      float s[WROWS];
+#pragma unroll
+      for (int i = 0; i < WROWS; ++i) s[i] = 0.f;
+      for (int d = 0; d < hd4; d += 4) {
+        const float4 k4 = *reinterpret_cast<const float4 *>(sK + lane * kst + d);
+#pragma unroll
+        for (int i = 0; i < WROWS; ++i)
+          if (i < live) {
+            const float4 q4 = *reinterpret_cast<const float4 *>(sQ + (warp + 4 * i) * hd4 + d);
+            s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+          }
+      }
+      const int key = kt * TILE + lane;
+#pragma unroll
+      for (int i = 0; i < WROWS; ++i)
+        if (i < live) {
+          const float x = key < limit[i] ? s[i] * sl2 : -INFINITY, mn = fmaxf(m[i], warp_max(x));
+          const float base = mn == -INFINITY ? 0.f : mn, f = exp2f(m[i] - base), p = exp2f(x - base);
+          m[i] = mn;
+          l[i] = l[i] * f + warp_sum(p);
+#pragma unroll
+          for (int j = 0; j < HJ; ++j) { acc[i][j].x *= f; acc[i][j].y *= f; acc[i][j].z *= f; acc[i][j].w *= f; }
+          sP[i * TILE + lane] = p;
+        }
+      __syncwarp();
+#pragma unroll 2
+      for (int k = 0; k < TILE; k += 4) {
+        float4 p4[WROWS];
+#pragma unroll
+        for (int i = 0; i < WROWS; ++i) p4[i] = i < live ? *reinterpret_cast<const float4 *>(sP + i * TILE + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < HJ; ++j) {
+          const int d = lane * 4 + 128 * j;
+          if (d < hd4) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              const float4 v4 = *reinterpret_cast<const float4 *>(sV + (k + kk) * hd4 + d);
+#pragma unroll
+              for (int i = 0; i < WROWS; ++i)
+                if (i < live) {
+                  const float p = kk == 0 ? p4[i].x : kk == 1 ? p4[i].y : kk == 2 ? p4[i].z : p4[i].w;
+                  acc[i][j].x = fmaf(p, v4.x, acc[i][j].x); acc[i][j].y = fmaf(p, v4.y, acc[i][j].y);
+                  acc[i][j].z = fmaf(p, v4.z, acc[i][j].z); acc[i][j].w = fmaf(p, v4.w, acc[i][j].w);
+                }
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    // ---- the whole block: its rows; a part of it: a partial result
+    const bool whole = pl.kt == 0 && kt1 == tiles;
+    float *slot = whole ? nullptr : paged_slot(a, c, pl.kt == 0);
+#pragma unroll
+    for (int i = 0; i < WROWS; ++i)
+      if (i < live) {
+        const int r = warp + 4 * i;
+        const float inv = whole ? (l[i] > 0.f ? 1.0f / l[i] : 0.f) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < HJ; ++j) {
+          const float e[4] = {acc[i][j].x * inv, acc[i][j].y * inv, acc[i][j].z * inv, acc[i][j].w * inv};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int d = lane * 4 + 128 * j + x;
+            if (d < hd) {
+              if (whole) ((T *)a.o)[(size_t)out_row[i] * a.ld_o + (size_t)out_head[i] * hd + d] = from_f<T>(e[x]);
+              else slot[(size_t)r * hd + d] = e[x];
+            }
+          }
+        }
+        if (lane == 0) {
+          if (!whole) { slot[(size_t)a.slot_rows * hd + r] = m[i]; slot[(size_t)a.slot_rows * (hd + 1) + r] = l[i]; }
+          else if (a.lse) a.lse[(size_t)out_row[i] * a.nH + out_head[i]] = l[i] > 0.f ? (m[i] + log2f(l[i])) / PAGED_LOG2E : -INFINITY;
+        }
+      }
+    u += kt1 - pl.kt;
+    if (u < end) paged::line_next(a.b, a.plan, pl);
+  }
+}
+
+// ---- join: one CTA per border between runs; it works when the border is the first one inside its block ------------------
+constexpr int JOIN_THREADS = 256;
+template <class T>
+__global__ void __launch_bounds__(JOIN_THREADS)
+paged_join_kernel(PagedAttnArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ long long red[33];
+  __shared__ paged::Place place;
+  const long long total = paged::line_total<JOIN_THREADS>(a.b, a.plan, red);
+  const int n = paged::line_ctas(total, a.n_cta, a.min_units), c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
+  if (c >= n || total == 0) return;
+  const long long u = paged::line_at(total, n, c);
+  if (u == paged::line_at(total, n, c - 1)) return;
+  paged::line_find<JOIN_THREADS>(a.b, a.plan, u, red, &place);
+  const paged::Place pl = place;
+  const long long first = u - pl.kt, last = first + a.plan.tiles(pl.q, pl.block);      // the block's units
+  if (pl.kt == 0 || paged::line_at(total, n, c - 1) > first) return;                   // not inside a block, or not the first border in it
+  int c1 = c;                                                                          // parts: CTAs c - 1 .. c1
+  while (c1 + 1 < n && paged::line_at(total, n, c1 + 1) < last) ++c1;
+  const float *part0 = paged_slot(a, c - 1, true);
+  const size_t step = 2 * paged_slot_floats(a.slot_rows, hd);
+  const int vecs = (hd + 3) / 4;
+  for (int i = blockIdx.y * JOIN_THREADS + tid; i < a.slot_rows * vecs; i += gridDim.y * JOIN_THREADS) {
+    const int r = i / vecs, d = (i - r * vecs) * 4;
+    int row, head, pos;
+    if (!paged_row(a, pl, r, row, head, pos)) continue;
+    const int parts = c1 - c + 2;
+    auto part = [&](int k) { return k == 0 ? part0 : paged_slot(a, c, false) + (size_t)(k - 1) * step; };
+    float mx = -INFINITY;
+    for (int k = 0; k < parts; ++k) mx = fmaxf(mx, part(k)[(size_t)a.slot_rows * hd + r]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const float *p = part(k);
+      const float w = exp2f(p[(size_t)a.slot_rows * hd + r] - base);
+      l += w * p[(size_t)a.slot_rows * (hd + 1) + r];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (d + x < hd) e[x] = fmaf(w, p[(size_t)r * hd + d + x], e[x]);
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (d + x < hd) ((T *)a.o)[(size_t)row * a.ld_o + (size_t)head * hd + d + x] = from_f<T>(e[x] * inv);
+    if (a.lse && d == 0) a.lse[(size_t)row * a.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
+  }
+}
+
+template <class T, int HJ>
+int simt_launch(b200_ctx *ctx, const PagedAttnArgs &a) {
+  const int hd4 = (a.b.hd + 3) & ~3;
+  const size_t smem = sizeof(float) * (size_t)(TILE * (hd4 + 4) + TILE * hd4 + ROWS * hd4 + ROWS * TILE);
+  static std::atomic<unsigned long long> attr{0};
+  const unsigned long long bit = 1ull << (ctx->device & 63);
+  if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_simt_kernel<T, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024)); attr.fetch_or(bit); }
+  B200_CUDA(ctx, launch_k(ctx, paged_attn_simt_kernel<T, HJ>, dim3((unsigned)a.n_cta), dim3(THREADS), smem, 0, a));
+  B200_LAUNCHED(ctx);
+  return B200_OK;
+}
+
+constexpr int MIN_UNITS = 4;
+
+}  // namespace
+
+int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt) {
+  if (a.n_cta < 2) return B200_OK;
+  const int work = a.slot_rows * ((a.b.hd + 3) / 4);
+  const dim3 grid((unsigned)(a.n_cta - 1), (unsigned)((work + 4 * JOIN_THREADS - 1) / (4 * JOIN_THREADS)));
+  if (dt == B200_BF16) B200_CUDA(ctx, launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a));
+  else B200_CUDA(ctx, launch_k(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a));
+  B200_LAUNCHED(ctx);
+  return B200_OK;
+}
+
+static size_t simt_workspace(const b200_ctx *ctx, size_t hd) { return (size_t)4 * ctx->sm_count * paged_slot_floats(ROWS, (int)hd) * sizeof(float); }
+
+extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, size_t n_heads, size_t *bytes) {
+  if (!ctx) return B200_ERR_INVALID;
+  PagedArgs a;
+  int rc = paged_args(ctx, cache, batch, &a);
+  if (rc) return rc;
+  B200_REQUIRE(ctx, bytes, "paged_attn_workspace: null pointer");
+  B200_REQUIRE(ctx, n_heads > 0 && n_heads <= 65536 && n_heads % cache->n_kv == 0, "paged_attn: n_heads must be a multiple of the cache's n_kv");
+  *bytes = simt_workspace(ctx, cache->head_dim);
+  return B200_OK;
+}
+
+extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, const void *q, size_t ld_q, void *o,
+                               size_t ld_o, float *lse, size_t n_heads, float scale, void *workspace, size_t workspace_bytes) {
+  if (!ctx) return B200_ERR_INVALID;
+  PagedAttnArgs a;
+  size_t need = 0;
+  int rc = paged_args(ctx, cache, batch, &a.b);
+  if (!rc) rc = b200_paged_attn_workspace(ctx, cache, batch, n_heads, &need);
+  if (rc) return rc;
+  if (cache->head_dim > 256) return b200_fail(ctx, B200_ERR_UNSUPPORTED, "paged_attn: head_dim above 256 has no kernel");
+  B200_REQUIRE(ctx, std::isfinite(scale) && scale >= 0.f, "paged_attn: scale must be finite and not negative (0: 1 / sqrt(head_dim))");
+  if (batch->n_seq == 0 || batch->rows == 0) return B200_OK;
+  B200_REQUIRE(ctx, q && o, "paged_attn: null pointer");
+  B200_REQUIRE(ctx, ld_q >= n_heads * cache->head_dim && ld_o >= n_heads * cache->head_dim, "paged_attn: a row stride is shorter than the row");
+  B200_REQUIRE(ctx, workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0, "paged_attn: the workspace is smaller than b200_paged_attn_workspace says, or not 16-byte aligned");
+  DeviceGuard guard(ctx);
+  B200_REQUIRE(ctx, guard.ok, "paged_attn: the context's device cannot be selected");
+  a.k = cache->k; a.v = cache->v; a.q = q; a.o = o; a.lse = lse; a.ws = (float *)workspace;
+  a.ld_q = (long long)ld_q; a.ld_o = (long long)ld_o; a.nH = (int)n_heads;
+  a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)cache->head_dim);
+  a.plan = paged::Plan{(int)(n_heads / cache->n_kv), 0, ROWS, TILE, 0, 0x7fffffff};
+  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
+  const bool big = cache->head_dim > 128;
+  if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
+  else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);
+  if (rc) return rc;
+  return paged_join_launch(ctx, a, cache->dtype);
+}
+
+// Test hooks, on the host, over host arrays: what the kernels' own index code reaches.
+// out = {largest row + 1, largest slot + 1, smallest row, smallest slot, status}; slots count page * page_size + offset.
+extern "C" int b200_internal_paged_probe(const b200_paged_cache *cache, const b200_paged_batch *batch, long long *out) {
+  int status = 0;
+  b200_ctx ctx;
+  PagedArgs a;
+  if (int rc = paged_args(&ctx, cache, batch, &a)) return rc;
+  a.status = &status;
+  for (int i = 0; i < 4; ++i) out[i] = 0;
+  for (int s = 0; s < a.n_seq; ++s) {
+    const paged::Seq q = paged::load_seq(a, s);
+    if (q.ql > 0) { out[0] = std::max(out[0], (long long)q.q0 + q.ql); out[2] = std::min(out[2], (long long)q.q0); }
+    for (int pos = 0; pos < q.len; ++pos) {
+      const int page = paged::page_of(a, s, pos);
+      if (page < 0) continue;
+      const long long slot = (long long)page * a.page_size + pos % a.page_size;
+      out[1] = std::max(out[1], slot + 1); out[3] = std::min(out[3], slot);
+    }
+  }
+  out[4] = status;
+  return B200_OK;
+}
+// Steps through the runs of all CTAs; writes (CTA, sequence, KV head, block, tile, whole block) per tile, returns how many.
+extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile, int lo,
+                                               int hi, int n_cta, int min_units, int *out, long long room) {
+  int status = 0;
+  b200_ctx ctx;
+  PagedArgs a;
+  if (paged_args(&ctx, cache, batch, &a)) return -1;
+  a.status = &status;
+  const paged::Plan p{G, tokens, rows, tile, lo, hi};
+  long long total = 0, n_out = 0;
+  for (int s = 0; s < a.n_seq; ++s) total += paged::seq_units(a, p, s);
+  if (total == 0) return 0;
+  const int n = paged::line_ctas(total, n_cta, min_units);
+  for (int c = 0; c < n; ++c) {
+    long long u = paged::line_at(total, n, c), at = 0;
+    const long long end = paged::line_at(total, n, c + 1);
+    if (u == end) continue;
+    int s = 0;
+    while (true) { const long long m = paged::seq_units(a, p, s); if (u < at + m) break; at += m; ++s; }
+    paged::Place pl = paged::place_in(a, p, s, paged::seq_units(a, p, s), u - at);
+    while (u < end) {
+      const int tiles = p.tiles(pl.q, pl.block), kt1 = (int)std::min((long long)tiles, pl.kt + (end - u));
+      for (int t = pl.kt; t < kt1; ++t, ++n_out)
+        if (n_out < room) { const int v[6] = {c, pl.seq, pl.kvh, pl.block, t, pl.kt == 0 && kt1 == tiles}; std::copy(v, v + 6, out + 6 * n_out); }
+      u += kt1 - pl.kt;
+      if (u < end) paged::line_next(a, p, pl);
+    }
+  }
+  return n_out;
+}

@@ -1,0 +1,41 @@
+// Shared by the attention kernels over a paged cache: arguments, the layout of partial results, the launcher of the join.
+#pragma once
+#include "paged_common.cuh"
+
+struct PagedAttnArgs {
+  PagedArgs b;
+  paged::Plan plan;
+  const void *k, *v, *q;
+  void *o;
+  float *lse, *ws;
+  long long ld_q, ld_o;
+  int nH, n_cta, min_units, slot_rows;   // slot_rows: rows of one partial result
+  float scale;
+};
+
+constexpr float PAGED_LOG2E = 1.4426950408889634f;
+
+// Partial result of a block: [slot_rows][hd] output in units of 2^maximum, then [slot_rows] maxima (log2 units), [slot_rows] sums.
+// CTA c owns two: slot 2c for a block that began before its run, 2c + 1 for one that begins in it and ends behind it.
+__host__ __device__ __forceinline__ size_t paged_slot_floats(int slot_rows, int hd) { return (size_t)slot_rows * (hd + 2); }
+__device__ __forceinline__ float *paged_slot(const PagedAttnArgs &a, int cta, bool begins) {
+  return a.ws + (size_t)(2 * cta + (begins ? 1 : 0)) * paged_slot_floats(a.slot_rows, a.b.hd);
+}
+// (row of q / o, query head) of row r of a block; false where the block has no such row.
+__device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::Place &pl, int r, int &row, int &head, int &pos) {
+  int tok, g;
+  if (a.plan.rows_per_block) {
+    const long long f = (long long)pl.block * a.plan.rows_per_block + r;
+    tok = (int)(f / a.plan.G); g = (int)(f - (long long)tok * a.plan.G);
+  } else {
+    const int t = r / a.plan.G;
+    tok = pl.block * a.plan.tokens_per_block + t; g = r - t * a.plan.G;
+    if (t >= a.plan.tokens_per_block) return false;
+  }
+  row = pl.q.q0 + tok; head = pl.kvh * a.plan.G + g; pos = pl.q.base + tok;
+  return tok < pl.q.ql;
+}
+
+int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt);
+bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t ld_q, const void *o, size_t ld_o);
+int paged_attn_few_launch(b200_ctx *ctx, const PagedAttnArgs &a);

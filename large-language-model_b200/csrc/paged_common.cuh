@@ -1,0 +1,167 @@
+// What the kernels over a paged key/value cache share: the ragged batch, its checks on the device, and the division of its
+// attention work into equal runs.
+//
+// The lengths and the page table live on the device (a captured step replays with new ones), so the host knows only upper
+// bounds and nothing the kernels read may be trusted: every length is clamped to the arrays it indexes, every page id is
+// compared with the page count before it is used, and the first violation is recorded in the context's status word.
+#pragma once
+#include "common.cuh"
+
+constexpr int PAGED_BAD_BATCH = 3;      // status code: a page id or a length of the batch is out of range
+
+struct PagedArgs {
+  const int *q_start, *kv_len, *table;  // [n_seq + 1], [n_seq], [n_seq, table_ld]
+  int n_seq, table_ld, rows, max_q;
+  int page_size, n_pages, n_kv, hd;
+  long long page_stride, token_stride, head_stride;   // elements
+  int *status;
+};
+
+struct DeviceGuard {                    // entry points may be called with another device current
+  int prev = -1;
+  bool ok = true;
+  explicit DeviceGuard(const b200_ctx *ctx) {
+    if (cudaGetDevice(&prev) != cudaSuccess) { ok = false; return; }
+    if (prev == ctx->device) prev = -1;
+    else ok = cudaSetDevice(ctx->device) == cudaSuccess;
+  }
+  ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+// Host checks of the two descriptors; fills `a`.
+int paged_args(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, PagedArgs *a);
+
+namespace paged {
+
+struct Seq { int q0, ql, base, len; };  // first row, rows, position of row 0, cached positions
+
+// The checks and the stepping below also compile for the host, where the CPU tests run them.
+__host__ __device__ __forceinline__ void bad_batch(const PagedArgs &a) {
+#ifdef __CUDA_ARCH__
+  atomicCAS(a.status, 0, PAGED_BAD_BATCH);
+#else
+  *a.status = PAGED_BAD_BATCH;
+#endif
+}
+__host__ __device__ __forceinline__ int lesser(int a, int b) { return a < b ? a : b; }
+__host__ __device__ __forceinline__ int greater(int a, int b) { return a > b ? a : b; }
+
+__host__ __device__ __forceinline__ Seq load_seq(const PagedArgs &a, int s) {
+  const int r0 = a.q_start[s], r1 = a.q_start[s + 1], l = a.kv_len[s];
+  const long long room = (long long)a.table_ld * a.page_size;
+  Seq q;
+  q.q0 = lesser(greater(r0, 0), a.rows);
+  const int q1 = lesser(greater(r1, q.q0), a.rows), n = q1 - q.q0;
+  q.ql = lesser(n, a.max_q);
+  q.len = l < 0 ? 0 : l > room ? (int)room : l;
+  q.base = q.len - n;
+  if (q.q0 != r0 || q1 != r1 || q.ql != n || q.len != l) bad_batch(a);
+  return q;
+}
+// Page of position `pos`, or -1 (recorded) when the table holds an id outside the cache.
+__host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int pos) {
+  const int id = a.table[(long long)s * a.table_ld + pos / a.page_size];
+  if ((unsigned)id < (unsigned)a.n_pages) return id;
+  bad_batch(a);
+  return -1;
+}
+
+// ---- division of the work ---------------------------------------------------------------------------------------------
+// A sequence's rows (token, query head of the group) are cut into blocks; a block walks the key tiles its last row can see.
+// All (sequence, KV head, block, tile) in this order form one line of `total` units, and CTA c of n works on
+// [c * total / n, (c + 1) * total / n): every SM gets the same number of tiles whatever the lengths are.  A block that
+// crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
+struct Plan {
+  int G, tokens_per_block, rows_per_block;   // rows_per_block > 0: blocks of consecutive rows; else blocks of whole tokens
+  int tile, min_rows, max_rows;              // keys per tile; only sequences with min_rows <= rows <= max_rows take part
+  __host__ __device__ __forceinline__ bool takes(int ql) const { const long long r = (long long)ql * G; return ql > 0 && r >= min_rows && r <= max_rows; }
+  __host__ __device__ __forceinline__ int blocks(int ql) const {
+    return rows_per_block ? (int)(((long long)ql * G + rows_per_block - 1) / rows_per_block) : (ql + tokens_per_block - 1) / tokens_per_block;
+  }
+  __host__ __device__ __forceinline__ int tiles(const Seq &q, int block) const {
+    const long long end = rows_per_block ? ((long long)(block + 1) * rows_per_block - 1) / G + 1 : (long long)(block + 1) * tokens_per_block;
+    const int last = (int)(end < q.ql ? end : q.ql) - 1;
+    const int seen = lesser(greater(q.base + last + 1, 0), q.len);
+    return greater(1, (seen + tile - 1) / tile);   // a block that sees nothing still writes its empty rows
+  }
+};
+struct Place { int seq, kvh, block, kt; Seq q; };   // a position on the line: tile kt of a block
+
+__host__ __device__ __forceinline__ long long seq_units(const PagedArgs &a, const Plan &p, int s) {
+  const Seq q = load_seq(a, s);
+  if (!p.takes(q.ql)) return 0;
+  long long u = 0;
+  for (int b = p.blocks(q.ql) - 1; b >= 0; --b) u += p.tiles(q, b);
+  return u * a.n_kv;
+}
+
+// Unit `rest` of sequence s, which has `units`.
+__host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Plan &p, int s, long long units, long long rest) {
+  const long long per_head = units / a.n_kv;
+  Place pl;
+  pl.seq = s; pl.q = load_seq(a, s); pl.kvh = (int)(rest / per_head); rest -= pl.kvh * per_head;
+  int b = 0, t = p.tiles(pl.q, 0);
+  while (rest >= t) { rest -= t; t = p.tiles(pl.q, ++b); }
+  pl.block = b; pl.kt = (int)rest;
+  return pl;
+}
+
+// Exclusive prefix over the CTA's threads and the CTA total; `red` is shared [33].  All threads must call.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long *red, long long &sum) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+  __syncthreads();
+  if (lane == 31) red[w] = inc;
+  __syncthreads();
+  long long before = 0; sum = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) { if (i < w) before += red[i]; sum += red[i]; }
+  return before + inc - v;
+}
+
+// The line of this plan for at most n_max CTAs that get min_units at least (fewer CTAs take part otherwise).
+__host__ __device__ __forceinline__ int line_ctas(long long total, int n_max, int min_units) {
+  const long long n = (total + min_units - 1) / min_units;
+  return n < 1 ? 1 : n < n_max ? (int)n : n_max;
+}
+__host__ __device__ __forceinline__ long long line_at(long long total, int n, int c) { return total * c / n; }
+
+template <int THREADS>
+__device__ long long line_total(const PagedArgs &a, const Plan &p, long long *red) {
+  long long mine = 0, sum;
+  for (int s = threadIdx.x; s < a.n_seq; s += THREADS) mine += seq_units(a, p, s);
+  block_scan<THREADS>(mine, red, sum);
+  return sum;
+}
+// Finds unit u (0 <= u < total) and leaves it in *out (shared).  All threads must call; ends with a barrier.
+template <int THREADS>
+__device__ void line_find(const PagedArgs &a, const Plan &p, long long u, long long *red, Place *out) {
+  long long done = 0;
+  for (int s0 = 0; s0 < a.n_seq; s0 += THREADS) {
+    const int s = s0 + (int)threadIdx.x;
+    const long long mine = s < a.n_seq ? seq_units(a, p, s) : 0;
+    long long sum;
+    const long long at = done + block_scan<THREADS>(mine, red, sum);
+    if (u >= at && u < at + mine) *out = place_in(a, p, s, mine, u - at);
+    done += sum;
+    if (done > u) break;                     // the same for all threads
+  }
+  __syncthreads();
+}
+// The start of the next block on the line.
+__host__ __device__ __forceinline__ void line_next(const PagedArgs &a, const Plan &p, Place &pl) {
+  pl.kt = 0;
+  if (++pl.block < p.blocks(pl.q.ql)) return;
+  pl.block = 0;
+  if (++pl.kvh < a.n_kv) return;
+  pl.kvh = 0;
+  while (++pl.seq < a.n_seq) {
+    pl.q = load_seq(a, pl.seq);
+    if (p.takes(pl.q.ql)) return;
+  }
+}
+
+}  // namespace paged
