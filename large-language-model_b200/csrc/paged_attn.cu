@@ -22,20 +22,19 @@ constexpr int THREADS = 128, ROWS = 32, TILE = 32, WROWS = ROWS / 4;
 template <class T, int HJ>
 __global__ void __launch_bounds__(THREADS)
 paged_attn_simt_kernel(PagedAttnArgs a) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();                     // behind the wait: the join may read the batch as soon as it starts
   extern __shared__ __align__(16) float smem[];
   __shared__ long long red[33];
   __shared__ paged::Place place;
   __shared__ int page_s[TILE];
   const int hd = a.b.hd, hd4 = (hd + 3) & ~3, kst = hd4 + 4, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float *sK = smem, *sV = sK + TILE * kst, *sQ = sV + TILE * hd4, *sP = sQ + ROWS * hd4 + warp * WROWS * TILE;
-  const long long total = paged::line_total<THREADS>(a.b, a.plan, red);
-  const int n = paged::line_ctas(total, a.n_cta, a.min_units), c = blockIdx.x;
-  if (c >= n || total == 0) return;
-  long long u = paged::line_at(total, n, c);
-  const long long end = paged::line_at(total, n, c + 1);
-  paged::line_find<THREADS>(a.b, a.plan, u, red, &place);
+  const int c = blockIdx.x;
+  const paged::Run run = paged::line_run<THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
+  long long u = run.u;
+  const long long end = run.end;
+  if (u == end) return;
   paged::Place pl = place;
   const float sl2 = a.scale * PAGED_LOG2E;
   while (u < end) {
@@ -165,16 +164,17 @@ constexpr int JOIN_THREADS = 256;
 template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(PagedAttnArgs a) {
-  pdl_launch_dependents();
-  pdl_wait();
   __shared__ long long red[33];
   __shared__ paged::Place place;
-  const long long total = paged::line_total<JOIN_THREADS>(a.b, a.plan, red);
-  const int n = paged::line_ctas(total, a.n_cta, a.min_units), c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
-  if (c >= n || total == 0) return;
-  const long long u = paged::line_at(total, n, c);
+  // The division is worked out while the kernel before still runs: it reads the batch alone, which was there before that kernel began.
+  const int c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
+  const paged::Run run = paged::line_run<JOIN_THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (c >= run.n || run.total == 0) return;
+  const long long u = run.u, total = run.total;
+  const int n = run.n;
   if (u == paged::line_at(total, n, c - 1)) return;
-  paged::line_find<JOIN_THREADS>(a.b, a.plan, u, red, &place);
   const paged::Place pl = place;
   const long long first = u - pl.kt, last = first + a.plan.tiles(pl.q, pl.block);      // the block's units
   if (pl.kt == 0 || paged::line_at(total, n, c - 1) > first) return;                   // not inside a block, or not the first border in it
@@ -230,13 +230,20 @@ int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt) {
   if (a.n_cta < 2) return B200_OK;
   const int work = a.slot_rows * ((a.b.hd + 3) / 4);
   const dim3 grid((unsigned)(a.n_cta - 1), (unsigned)((work + 4 * JOIN_THREADS - 1) / (4 * JOIN_THREADS)));
-  if (dt == B200_BF16) B200_CUDA(ctx, launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a));
-  else B200_CUDA(ctx, launch_k(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a));
+  const bool pdl = ctx->pdl;
+  ctx->pdl = true;                             // the join's set-up overlaps the end of the kernel before it
+  const cudaError_t e = dt == B200_BF16 ? launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a)
+                                        : launch_k(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a);
+  ctx->pdl = pdl;
+  B200_CUDA(ctx, e);
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
 
-static size_t simt_workspace(const b200_ctx *ctx, size_t hd) { return (size_t)4 * ctx->sm_count * paged_slot_floats(ROWS, (int)hd) * sizeof(float); }
+// Each kernel leaves two partial results per CTA; the kernels of one call follow each other, so they share the room.
+static size_t partial_bytes(const b200_ctx *ctx, int ctas_per_sm, int slot_rows, size_t hd) {
+  return (size_t)2 * ctas_per_sm * ctx->sm_count * paged_slot_floats(slot_rows, (int)hd) * sizeof(float);
+}
 
 extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, size_t n_heads, size_t *bytes) {
   if (!ctx) return B200_ERR_INVALID;
@@ -245,7 +252,7 @@ extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *
   if (rc) return rc;
   B200_REQUIRE(ctx, bytes, "paged_attn_workspace: null pointer");
   B200_REQUIRE(ctx, n_heads > 0 && n_heads <= 65536 && n_heads % cache->n_kv == 0, "paged_attn: n_heads must be a multiple of the cache's n_kv");
-  *bytes = simt_workspace(ctx, cache->head_dim);
+  *bytes = partial_bytes(ctx, 2, ROWS, cache->head_dim);
   return B200_OK;
 }
 
@@ -268,7 +275,18 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
   a.k = cache->k; a.v = cache->v; a.q = q; a.o = o; a.lse = lse; a.ws = (float *)workspace;
   a.ld_q = (long long)ld_q; a.ld_o = (long long)ld_o; a.nH = (int)n_heads;
   a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)cache->head_dim);
-  a.plan = paged::Plan{(int)(n_heads / cache->n_kv), 0, ROWS, TILE, 0, 0x7fffffff};
+  const int G = (int)(n_heads / cache->n_kv);
+  int few = 0;                                  // sequences of up to this many rows are taken by the few-row kernel
+  if (paged_attn_few_supported(cache, q, ld_q, o, ld_o)) {
+    // A lone sequence or two with many rows are not worth a launch that will find nothing (each kernel is right for any row count).
+    const long long most = (long long)a.b.max_q * G;
+    if (most <= PAGED_FEW_ROWS || a.b.n_seq > 2) {
+      rc = paged_attn_few_launch(ctx, a, G);
+      if (rc || most <= PAGED_FEW_ROWS) return rc;
+      few = PAGED_FEW_ROWS;
+    }
+  }
+  a.plan = paged::Plan{G, 0, ROWS, TILE, few + 1, 0x7fffffff};
   a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
   const bool big = cache->head_dim > 128;
   if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);

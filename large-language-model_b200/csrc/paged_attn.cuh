@@ -13,6 +13,7 @@ struct PagedAttnArgs {
   float scale;
 };
 
+constexpr int PAGED_FEW_ROWS = 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 // Partial result of a block: [slot_rows][hd] output in units of 2^maximum, then [slot_rows] maxima (log2 units), [slot_rows] sums.
@@ -38,4 +39,4 @@ __device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::P
 
 int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt);
 bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t ld_q, const void *o, size_t ld_o);
-int paged_attn_few_launch(b200_ctx *ctx, const PagedAttnArgs &a);
+int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G);   // the kernel and its join

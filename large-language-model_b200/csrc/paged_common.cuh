@@ -122,34 +122,44 @@ __device__ __forceinline__ long long block_scan(long long v, long long *red, lon
   return before + inc - v;
 }
 
-// The line of this plan for at most n_max CTAs that get min_units at least (fewer CTAs take part otherwise).
+// CTAs that take part: at most n_max, and few enough that each gets min_units.
 __host__ __device__ __forceinline__ int line_ctas(long long total, int n_max, int min_units) {
   const long long n = (total + min_units - 1) / min_units;
   return n < 1 ? 1 : n < n_max ? (int)n : n_max;
 }
 __host__ __device__ __forceinline__ long long line_at(long long total, int n, int c) { return total * c / n; }
 
+struct Run { long long u, end, total; int n; };          // units [u, end) of CTA c; n CTAs take part
+
+// The run of CTA c, and the place of unit u in *out (shared) unless the run is empty.  All threads must call; ends with a barrier.
 template <int THREADS>
-__device__ long long line_total(const PagedArgs &a, const Plan &p, long long *red) {
-  long long mine = 0, sum;
-  for (int s = threadIdx.x; s < a.n_seq; s += THREADS) mine += seq_units(a, p, s);
-  block_scan<THREADS>(mine, red, sum);
-  return sum;
-}
-// Finds unit u (0 <= u < total) and leaves it in *out (shared).  All threads must call; ends with a barrier.
-template <int THREADS>
-__device__ void line_find(const PagedArgs &a, const Plan &p, long long u, long long *red, Place *out) {
-  long long done = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += THREADS) {
-    const int s = s0 + (int)threadIdx.x;
-    const long long mine = s < a.n_seq ? seq_units(a, p, s) : 0;
-    long long sum;
-    const long long at = done + block_scan<THREADS>(mine, red, sum);
-    if (u >= at && u < at + mine) *out = place_in(a, p, s, mine, u - at);
-    done += sum;
-    if (done > u) break;                     // the same for all threads
+__device__ Run line_run(const PagedArgs &a, const Plan &p, int c, int n_max, int min_units, long long *red, Place *out) {
+  const int tid = (int)threadIdx.x;
+  const long long first = tid < a.n_seq ? seq_units(a, p, tid) : 0;
+  long long mine = first, total;
+  for (int s = tid + THREADS; s < a.n_seq; s += THREADS) mine += seq_units(a, p, s);
+  long long at = block_scan<THREADS>(mine, red, total);
+  Run r;
+  r.total = total; r.n = line_ctas(total, n_max, min_units);
+  r.u = r.end = 0;
+  if (total == 0 || c >= r.n) return r;
+  r.u = line_at(total, r.n, c); r.end = line_at(total, r.n, c + 1);
+  if (a.n_seq <= THREADS) {                                // each thread has one sequence: the scan above is the line
+    if (r.u >= at && r.u < at + mine) *out = place_in(a, p, tid, mine, r.u - at);
+  } else {
+    long long done = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += THREADS) {
+      const int s = s0 + tid;
+      const long long m = s0 == 0 ? first : s < a.n_seq ? seq_units(a, p, s) : 0;
+      long long sum;
+      at = done + block_scan<THREADS>(m, red, sum);
+      if (r.u >= at && r.u < at + m) *out = place_in(a, p, s, m, r.u - at);
+      done += sum;
+      if (done > r.u) break;                               // the same for all threads
+    }
   }
   __syncthreads();
+  return r;
 }
 // The start of the next block on the line.
 __host__ __device__ __forceinline__ void line_next(const PagedArgs &a, const Plan &p, Place &pl) {
