@@ -184,7 +184,8 @@ paged_join_kernel(PagedAttnArgs a) {
   const size_t step = 2 * paged_slot_floats(a.slot_rows, hd);
   const int vecs = (hd + 3) / 4;
   for (int i = blockIdx.y * JOIN_THREADS + tid; i < a.slot_rows * vecs; i += gridDim.y * JOIN_THREADS) {
-    const int r = i / vecs, d = (i - r * vecs) * 4;
+    const int r = a.columns ? i % a.slot_rows : i / vecs, v = a.columns ? i / a.slot_rows : i - r * vecs, d = v * 4;
+    const size_t at = a.columns ? ((size_t)v * a.slot_rows + r) * 4 : (size_t)r * hd + d;
     int row, head, pos;
     if (!paged_row(a, pl, r, row, head, pos)) continue;
     const int parts = c1 - c + 2;
@@ -197,10 +198,12 @@ paged_join_kernel(PagedAttnArgs a) {
     for (int k = 0; k < parts; ++k) {
       const float *p = part(k);
       const float w = exp2f(p[(size_t)a.slot_rows * hd + r] - base);
-      l += w * p[(size_t)a.slot_rows * (hd + 1) + r];
+      if (w > 0.f) {
+        l += w * p[(size_t)a.slot_rows * (hd + 1) + r];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (d + x < hd) e[x] = fmaf(w, p[(size_t)r * hd + d + x], e[x]);
+        for (int x = 0; x < 4; ++x)
+          if (d + x < hd) e[x] = fmaf(w, p[at + x], e[x]);
+      }
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
 #pragma unroll
@@ -252,7 +255,7 @@ extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *
   if (rc) return rc;
   B200_REQUIRE(ctx, bytes, "paged_attn_workspace: null pointer");
   B200_REQUIRE(ctx, n_heads > 0 && n_heads <= 65536 && n_heads % cache->n_kv == 0, "paged_attn: n_heads must be a multiple of the cache's n_kv");
-  *bytes = partial_bytes(ctx, 2, ROWS, cache->head_dim);
+  *bytes = std::max(partial_bytes(ctx, 2, ROWS, cache->head_dim), cache->dtype == B200_BF16 && cache->head_dim <= 128 ? partial_bytes(ctx, 1, 256, cache->head_dim) : 0);
   return B200_OK;
 }
 
@@ -286,8 +289,9 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
       few = PAGED_FEW_ROWS;
     }
   }
+  if (paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o)) return paged_attn_tc_launch(ctx, a, G, few + 1);
   a.plan = paged::Plan{G, 0, ROWS, TILE, few + 1, 0x7fffffff};
-  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
+  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS; a.columns = 0;
   const bool big = cache->head_dim > 128;
   if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
   else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);

@@ -9,7 +9,7 @@ struct PagedAttnArgs {
   void *o;
   float *lse, *ws;
   long long ld_q, ld_o;
-  int nH, n_cta, min_units, slot_rows;   // slot_rows: rows of one partial result
+  int nH, n_cta, min_units, slot_rows, columns;   // slot_rows: rows of one partial result
   float scale;
 };
 
@@ -17,7 +17,8 @@ constexpr int PAGED_FEW_ROWS = 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 // Partial result of a block: [slot_rows][hd] output in units of 2^maximum, then [slot_rows] maxima (log2 units), [slot_rows] sums.
-// CTA c owns two: slot 2c for a block that began before its run, 2c + 1 for one that begins in it and ends behind it.
+// With `columns` the output is laid out [hd / 4][slot_rows][4] instead (threads that each own a row write whole segments).
+// A part whose maximum is -inf saw no key; its output is not read.  CTA c owns two: slot 2c for a block that began before its run, 2c + 1 for one that begins in it and ends behind it.
 __host__ __device__ __forceinline__ size_t paged_slot_floats(int slot_rows, int hd) { return (size_t)slot_rows * (hd + 2); }
 __device__ __forceinline__ float *paged_slot(const PagedAttnArgs &a, int cta, bool begins) {
   return a.ws + (size_t)(2 * cta + (begins ? 1 : 0)) * paged_slot_floats(a.slot_rows, a.b.hd);
@@ -29,9 +30,10 @@ __device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::P
     const long long f = (long long)pl.block * a.plan.rows_per_block + r;
     tok = (int)(f / a.plan.G); g = (int)(f - (long long)tok * a.plan.G);
   } else {
-    const int t = r / a.plan.G;
-    tok = pl.block * a.plan.tokens_per_block + t; g = r - t * a.plan.G;
-    if (t >= a.plan.tokens_per_block) return false;
+    // two tiles of 128 rows, each of whole tokens
+    const int half = a.plan.tokens_per_block / 2, t = (r & 127) / a.plan.G;
+    tok = pl.block * a.plan.tokens_per_block + (r >> 7) * half + t; g = (r & 127) - t * a.plan.G;
+    if (t >= half) return false;
   }
   row = pl.q.q0 + tok; head = pl.kvh * a.plan.G + g; pos = pl.q.base + tok;
   return tok < pl.q.ql;
@@ -40,3 +42,5 @@ __device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::P
 int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt);
 bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t ld_q, const void *o, size_t ld_o);
 int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G);   // the kernel and its join
+bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const void *q, size_t ld_q, const void *o, size_t ld_o);
+int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs a, int G, int min_rows);   // the kernel and its join
