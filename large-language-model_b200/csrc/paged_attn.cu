@@ -32,13 +32,12 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
   float *sK = smem, *sV = sK + TILE * kst, *sQ = sV + TILE * hd4, *sP = sQ + ROWS * hd4 + warp * WROWS * TILE;
   const int c = blockIdx.x;
   const paged::Run run = paged::line_run<THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
-  long long u = run.u;
-  const long long end = run.end;
-  if (u == end) return;
-  paged::Place pl = place;
+  if (tid == 0) paged_write_head(a, run, place, c);
+  if (run.u == run.end) return;
+  paged::Walk w;
   const float sl2 = a.scale * PAGED_LOG2E;
-  while (u < end) {
-    const int tiles = a.plan.tiles(pl.q, pl.block), kt1 = (int)min((long long)tiles, pl.kt + (end - u));
+  for (w.start(a.plan, place, run.end); w.more; w.next(a.b, a.plan, run.end)) {
+    const paged::Place &pl = w.pl;
     // ---- queries of the block, rows that do not exist as zeros
     __syncthreads();
     for (int i = tid; i < ROWS * hd4; i += THREADS) {
@@ -61,7 +60,7 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int j = 0; j < HJ; ++j) acc[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int kt = pl.kt; kt < kt1; ++kt) {
+    for (int kt = pl.kt; kt < w.k1; ++kt) {
       __syncthreads();
       if (tid < TILE) {
         const int pos = kt * TILE + tid;
@@ -130,7 +129,7 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
       __syncwarp();
     }
     // ---- the whole block: its rows; a part of it: a partial result
-    const bool whole = pl.kt == 0 && kt1 == tiles;
+    const bool whole = w.whole();
     float *slot = whole ? nullptr : paged_slot(a, c, pl.kt == 0);
 #pragma unroll
     for (int i = 0; i < WROWS; ++i)
@@ -154,62 +153,95 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
           else if (a.lse) a.lse[(size_t)out_row[i] * a.nH + out_head[i]] = l[i] > 0.f ? (m[i] + log2f(l[i])) / PAGED_LOG2E : -INFINITY;
         }
       }
-    u += kt1 - pl.kt;
-    if (u < end) paged::line_next(a.b, a.plan, pl);
   }
 }
 
-// ---- join: one CTA per border between runs; it works when the border is the first one inside its block ------------------
-constexpr int JOIN_THREADS = 256;
+// ---- join: one CTA column per border between runs; it works when the border is the first one inside its block ------------
+// A thread owns four dimensions of a row and adds its parts in CTA order, the loads of four parts in flight at once (chains of
+// dependent loads made this kernel 40 to 70 us long).  With more than eight parts the CTA's eight warps share them out and add their sums.
+constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
 template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(PagedAttnArgs a) {
-  __shared__ long long red[33];
-  __shared__ paged::Place place;
-  // The division is worked out while the kernel before still runs: it reads the batch alone, which was there before that kernel began.
-  const int c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
-  const paged::Run run = paged::line_run<JOIN_THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
   pdl_wait();
   pdl_launch_dependents();
-  if (c >= run.n || run.total == 0) return;
-  const long long u = run.u, total = run.total;
-  const int n = run.n;
-  if (u == paged::line_at(total, n, c - 1)) return;
-  const paged::Place pl = place;
-  const long long first = u - pl.kt, last = first + a.plan.tiles(pl.q, pl.block);      // the block's units
-  if (pl.kt == 0 || paged::line_at(total, n, c - 1) > first) return;                   // not inside a block, or not the first border in it
-  int c1 = c;                                                                          // parts: CTAs c - 1 .. c1
-  while (c1 + 1 < n && paged::line_at(total, n, c1 + 1) < last) ++c1;
-  const float *part0 = paged_slot(a, c - 1, true);
+  __shared__ float sh_m[JOIN_WARPS][32], sh_l[JOIN_WARPS][32];
+  __shared__ float4 sh_e[JOIN_WARPS][32];
+  const int c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
+  const JoinHead *head_ = paged_head(a, c);
+  const int parts = head_->parts;
+  if (parts == 0) return;
+  const paged::Place pl = head_->pl;
+  const float *part0 = paged_slot(a, c - 1, true), *part1 = paged_slot(a, c, false);
   const size_t step = 2 * paged_slot_floats(a.slot_rows, hd);
-  const int vecs = (hd + 3) / 4;
-  for (int i = blockIdx.y * JOIN_THREADS + tid; i < a.slot_rows * vecs; i += gridDim.y * JOIN_THREADS) {
+  const int vecs = (hd + 3) / 4, items = a.slot_rows * vecs, groups = parts > 8 ? JOIN_WARPS : 1, width = JOIN_THREADS / groups;
+  const int group = tid / width, k0 = (int)((long long)parts * group / groups), k1 = (int)((long long)parts * (group + 1) / groups);
+  for (int i0 = blockIdx.y * width; i0 < items; i0 += gridDim.y * width) {
+    const int i = i0 + tid % width;
     const int r = a.columns ? i % a.slot_rows : i / vecs, v = a.columns ? i / a.slot_rows : i - r * vecs, d = v * 4;
     const size_t at = a.columns ? ((size_t)v * a.slot_rows + r) * 4 : (size_t)r * hd + d;
-    int row, head, pos;
-    if (!paged_row(a, pl, r, row, head, pos)) continue;
-    const int parts = c1 - c + 2;
-    auto part = [&](int k) { return k == 0 ? part0 : paged_slot(a, c, false) + (size_t)(k - 1) * step; };
-    float mx = -INFINITY;
-    for (int k = 0; k < parts; ++k) mx = fmaxf(mx, part(k)[(size_t)a.slot_rows * hd + r]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float *p = part(k);
-      const float w = exp2f(p[(size_t)a.slot_rows * hd + r] - base);
-      if (w > 0.f) {
-        l += w * p[(size_t)a.slot_rows * (hd + 1) + r];
+    int row = 0, head = 0, pos = 0;
+    const bool has = i < items && paged_row(a, pl, r, row, head, pos);
+    const bool vec = hd % 4 == 0;
+    float mx = -INFINITY, l = 0.f, e[4] = {0.f, 0.f, 0.f, 0.f};
+    if (has) {
+      const size_t at_m = (size_t)a.slot_rows * hd + r, at_l = at_m + a.slot_rows;
+      for (int k = k0; k < k1; k += 4) {
+        float m4[4], l4[4], e4[4][4], top = mx;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (d + x < hd) e[x] = fmaf(w, p[at + x], e[x]);
+        for (int j = 0; j < 4; ++j) {
+          const float *p = k + j == 0 ? part0 : part1 + (size_t)(k + j - 1) * step;
+          const bool in = k + j < k1;
+          m4[j] = in ? p[at_m] : -INFINITY;
+          l4[j] = in ? p[at_l] : 0.f;
+          if (vec) { const float4 x = in ? *reinterpret_cast<const float4 *>(p + at) : make_float4(0.f, 0.f, 0.f, 0.f); e4[j][0] = x.x; e4[j][1] = x.y; e4[j][2] = x.z; e4[j][3] = x.w; }
+          else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e4[j][x] = in && d + x < hd ? p[at + x] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, m4[j]);
+        const float base = top == -INFINITY ? 0.f : top, f = exp2f(mx - base);
+        l *= f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) e[x] *= f;
+        mx = top;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float wt = exp2f(m4[j] - base);
+          if (wt > 0.f) {                                    // a part that saw no key holds anything
+            l = fmaf(wt, l4[j], l);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = fmaf(wt, e4[j][x], e[x]);
+          }
+        }
       }
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    if (groups > 1) {
+      const int lane = tid & 31;
+      __syncthreads();
+      sh_m[group][lane] = mx; sh_l[group][lane] = l; sh_e[group][lane] = make_float4(e[0], e[1], e[2], e[3]);
+      __syncthreads();
+      if (group == 0) {
+        for (int k = 0; k < JOIN_WARPS; ++k) mx = fmaxf(mx, sh_m[k][lane]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        l = e[0] = e[1] = e[2] = e[3] = 0.f;
+        for (int k = 0; k < JOIN_WARPS; ++k) {
+          const float wt = exp2f(sh_m[k][lane] - base);
+          const float4 x = sh_e[k][lane];
+          l = fmaf(wt, sh_l[k][lane], l);
+          e[0] = fmaf(wt, x.x, e[0]); e[1] = fmaf(wt, x.y, e[1]); e[2] = fmaf(wt, x.z, e[2]); e[3] = fmaf(wt, x.w, e[3]);
+        }
+      }
+    }
+    if (has && group == 0) {
+      const float inv = l > 0.f ? 1.0f / l : 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (d + x < hd) ((T *)a.o)[(size_t)row * a.ld_o + (size_t)head * hd + d + x] = from_f<T>(e[x] * inv);
-    if (a.lse && d == 0) a.lse[(size_t)row * a.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
+      for (int x = 0; x < 4; ++x)
+        if (d + x < hd) ((T *)a.o)[(size_t)row * a.ld_o + (size_t)head * hd + d + x] = from_f<T>(e[x] * inv);
+      if (a.lse && d == 0) a.lse[(size_t)row * a.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
+    }
   }
 }
 
@@ -232,7 +264,7 @@ constexpr int MIN_UNITS = 4;
 int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt) {
   if (a.n_cta < 2) return B200_OK;
   const int work = a.slot_rows * ((a.b.hd + 3) / 4);
-  const dim3 grid((unsigned)(a.n_cta - 1), (unsigned)((work + 4 * JOIN_THREADS - 1) / (4 * JOIN_THREADS)));
+  const dim3 grid((unsigned)(a.n_cta - 1), (unsigned)std::min(16, (work + JOIN_THREADS - 1) / JOIN_THREADS));
   const bool pdl = ctx->pdl;
   ctx->pdl = true;                             // the join's set-up overlaps the end of the kernel before it
   const cudaError_t e = dt == B200_BF16 ? launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a)
@@ -245,7 +277,7 @@ int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt) {
 
 // Each kernel leaves two partial results per CTA; the kernels of one call follow each other, so they share the room.
 static size_t partial_bytes(const b200_ctx *ctx, int ctas_per_sm, int slot_rows, size_t hd) {
-  return (size_t)2 * ctas_per_sm * ctx->sm_count * paged_slot_floats(slot_rows, (int)hd) * sizeof(float);
+  return (size_t)ctas_per_sm * ctx->sm_count * (JOIN_HEAD_FLOATS + 2 * paged_slot_floats(slot_rows, (int)hd)) * sizeof(float);
 }
 
 extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, size_t n_heads, size_t *bytes) {
@@ -290,7 +322,7 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
     }
   }
   if (paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o)) return paged_attn_tc_launch(ctx, a, G, few + 1);
-  a.plan = paged::Plan{G, 0, ROWS, TILE, few + 1, 0x7fffffff};
+  a.plan = paged::Plan{G, 0, ROWS, TILE, 1, few + 1, 0x7fffffff};
   a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS; a.columns = 0;
   const bool big = cache->head_dim > 128;
   if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
@@ -321,33 +353,31 @@ extern "C" int b200_internal_paged_probe(const b200_paged_cache *cache, const b2
   out[4] = status;
   return B200_OK;
 }
-// Steps through the runs of all CTAs; writes (CTA, sequence, KV head, block, tile, whole block) per tile, returns how many.
-extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile, int lo,
-                                               int hi, int n_cta, int min_units, int *out, long long room) {
+// Steps through the runs of all CTAs; writes (CTA, sequence, KV head, block, tile, whole block, parts to join at the CTA's border) per tile, returns how many.
+extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile, int extra,
+                                               int lo, int hi, int n_cta, int min_units, int *out, long long room) {
   int status = 0;
   b200_ctx ctx;
   PagedArgs a;
   if (paged_args(&ctx, cache, batch, &a)) return -1;
   a.status = &status;
-  const paged::Plan p{G, tokens, rows, tile, lo, hi};
+  const paged::Plan p{G, tokens, rows, tile, extra, lo, hi};
   long long total = 0, n_out = 0;
   for (int s = 0; s < a.n_seq; ++s) total += paged::seq_units(a, p, s);
   if (total == 0) return 0;
   const int n = paged::line_ctas(total, n_cta, min_units);
   for (int c = 0; c < n; ++c) {
-    long long u = paged::line_at(total, n, c), at = 0;
-    const long long end = paged::line_at(total, n, c + 1);
-    if (u == end) continue;
+    const paged::Run run{paged::line_at(total, n, c), paged::line_at(total, n, c + 1), total, n};
+    if (run.u == run.end) continue;
+    long long at = 0;
     int s = 0;
-    while (true) { const long long m = paged::seq_units(a, p, s); if (u < at + m) break; at += m; ++s; }
-    paged::Place pl = paged::place_in(a, p, s, paged::seq_units(a, p, s), u - at);
-    while (u < end) {
-      const int tiles = p.tiles(pl.q, pl.block), kt1 = (int)std::min((long long)tiles, pl.kt + (end - u));
-      for (int t = pl.kt; t < kt1; ++t, ++n_out)
-        if (n_out < room) { const int v[6] = {c, pl.seq, pl.kvh, pl.block, t, pl.kt == 0 && kt1 == tiles}; std::copy(v, v + 6, out + 6 * n_out); }
-      u += kt1 - pl.kt;
-      if (u < end) paged::line_next(a, p, pl);
-    }
+    while (true) { const long long m = paged::seq_units(a, p, s); if (run.u < at + m) break; at += m; ++s; }
+    paged::Walk w;
+    w.start(p, paged::place_in(a, p, s, paged::seq_units(a, p, s), at, run.u), run.end);
+    const int parts = paged::parts_at(p, run, w.pl, c);
+    for (; w.more; w.next(a, p, run.end))
+      for (int t = w.pl.kt; t < w.k1; ++t, ++n_out)
+        if (n_out < room) { const int v[7] = {c, w.pl.seq, w.pl.kvh, w.pl.block, t, w.whole(), parts}; std::copy(v, v + 7, out + 7 * n_out); }
   }
   return n_out;
 }

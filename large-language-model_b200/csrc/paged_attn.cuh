@@ -7,7 +7,7 @@ struct PagedAttnArgs {
   paged::Plan plan;
   const void *k, *v, *q;
   void *o;
-  float *lse, *ws;
+  float *lse, *ws;                       // ws: the join's heads, then the partial results
   long long ld_q, ld_o;
   int nH, n_cta, min_units, slot_rows, columns;   // slot_rows: rows of one partial result
   float scale;
@@ -20,8 +20,19 @@ constexpr float PAGED_LOG2E = 1.4426950408889634f;
 // With `columns` the output is laid out [hd / 4][slot_rows][4] instead (threads that each own a row write whole segments).
 // A part whose maximum is -inf saw no key; its output is not read.  CTA c owns two: slot 2c for a block that began before its run, 2c + 1 for one that begins in it and ends behind it.
 __host__ __device__ __forceinline__ size_t paged_slot_floats(int slot_rows, int hd) { return (size_t)slot_rows * (hd + 2); }
+// What the join needs of the border before run c: written by CTA c (every CTA of the grid writes its own).
+struct alignas(16) JoinHead { int parts; paged::Place pl; };
+constexpr int JOIN_HEAD_FLOATS = 16;
+static_assert(sizeof(JoinHead) <= JOIN_HEAD_FLOATS * 4, "join head");
+__device__ __forceinline__ JoinHead *paged_head(const PagedAttnArgs &a, int cta) { return reinterpret_cast<JoinHead *>(a.ws + (size_t)cta * JOIN_HEAD_FLOATS); }
+__device__ __forceinline__ void paged_write_head(const PagedAttnArgs &a, const paged::Run &run, const paged::Place &pl, int c) {
+  JoinHead *h = paged_head(a, c);
+  const int parts = run.u == run.end ? 0 : paged::parts_at(a.plan, run, pl, c);
+  h->parts = parts;
+  if (parts) h->pl = pl;
+}
 __device__ __forceinline__ float *paged_slot(const PagedAttnArgs &a, int cta, bool begins) {
-  return a.ws + (size_t)(2 * cta + (begins ? 1 : 0)) * paged_slot_floats(a.slot_rows, a.b.hd);
+  return a.ws + (size_t)a.n_cta * JOIN_HEAD_FLOATS + (size_t)(2 * cta + (begins ? 1 : 0)) * paged_slot_floats(a.slot_rows, a.b.hd);
 }
 // (row of q / o, query head) of row r of a block; false where the block has no such row.
 __device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::Place &pl, int r, int &row, int &head, int &pos) {

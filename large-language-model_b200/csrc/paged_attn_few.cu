@@ -41,20 +41,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// A place on the line that steps tile by tile.
-struct Walk {
-  paged::Place pl;
-  int tiles;
-  long long u;
-  __device__ __forceinline__ void start(const PagedAttnArgs &a, const paged::Place &p, long long u0) { pl = p; u = u0; tiles = a.plan.tiles(pl.q, pl.block); }
-  __device__ __forceinline__ void step(const PagedAttnArgs &a, long long end) {
-    ++u;
-    if (++pl.kt < tiles || u >= end) return;
-    paged::line_next(a.b, a.plan, pl);
-    tiles = a.plan.tiles(pl.q, pl.block);
-  }
-};
-
 // MT: 16-row tiles.
 template <int HD, int MT>
 __global__ void __launch_bounds__(THREADS, 2)
@@ -70,21 +56,23 @@ paged_attn_few_kernel(PagedAttnArgs a) {
   __shared__ float sm_m[WARPS][16 * MT], sm_l[WARPS][16 * MT];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, c = blockIdx.x;
   const paged::Run run = paged::line_run<THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
+  if (tid == 0) paged_write_head(a, run, place, c);
   if (run.u == run.end) return;
   uint8_t *ring = smem + warp * STAGES * STAGE;
   const float sl2 = a.scale * PAGED_LOG2E;
 
   // ---- loads: this warp's slice of the walk's tile; the page ids of the next tile are fetched one tile ahead
-  Walk ld;
-  ld.start(a, place, run.u);
-  auto fetch_page = [&](const Walk &w) -> int {                // lane < 16: page of key `lane` of the slice, -1 past the end
-    const int pos = w.pl.kt * TILE + warp * SLICE + (lane & 15);
-    return w.u < run.end && pos < w.pl.q.len ? paged::page_of(a.b, w.pl.seq, pos) : -1;
+  paged::Walk ld;
+  ld.start(a.plan, place, run.end);
+  int ld_kt = ld.pl.kt;
+  auto fetch_page = [&]() -> int {                             // lane < 16: page of key `lane` of the slice, -1 past the end
+    const int pos = ld_kt * TILE + warp * SLICE + (lane & 15);
+    return ld.more && pos < ld.pl.q.len ? paged::page_of(a.b, ld.pl.seq, pos) : -1;
   };
-  int page = fetch_page(ld);
+  int page = fetch_page();
   auto load = [&](int stage) {
-    if (ld.u < run.end) {
-      const int pos = ld.pl.kt * TILE + warp * SLICE + (lane & 15);
+    if (ld.more) {
+      const int pos = ld_kt * TILE + warp * SLICE + (lane & 15);
       const long long off = page < 0 ? -1 : (long long)page * a.b.page_stride + (long long)(pos % a.b.page_size) * a.b.token_stride + (long long)ld.pl.kvh * a.b.head_stride;
       const uint32_t dst = smem_addr(ring + stage * STAGE);
 #pragma unroll
@@ -96,21 +84,19 @@ paged_attn_few_kernel(PagedAttnArgs a) {
         cp_async16(d, (const bf16 *)a.k + e, o >= 0);
         cp_async16(d + HALF, (const bf16 *)a.v + e, o >= 0);
       }
-      ld.step(a, run.end);
-      page = fetch_page(ld);
+      if (++ld_kt >= ld.k1) { ld.next(a.b, a.plan, run.end); ld_kt = 0; }
+      page = fetch_page();
     }
     cp_commit();
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load(s);
 
-  Walk w;
-  w.start(a, place, run.u);
+  paged::Walk w;
   int stage = 0;
-  while (w.u < run.end) {
+  for (w.start(a.plan, place, run.end); w.more; w.next(a.b, a.plan, run.end)) {
     // ---- a block: its queries in registers, rows that do not exist as zeros
-    const int kt0 = w.pl.kt, tiles = w.tiles;
-    const paged::Place pl = w.pl;
+    const paged::Place &pl = w.pl;
     uint32_t qf[MT][KS][4];
     int limit[MT][2];
 #pragma unroll
@@ -137,8 +123,7 @@ paged_attn_few_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
       mx[m][0] = mx[m][1] = -INFINITY; l[m][0] = l[m][1] = 0.f;
     }
-    const int n_tiles = (int)min((long long)(tiles - kt0), run.end - w.u);
-    for (int i = 0; i < n_tiles; ++i) {
+    for (int kt = pl.kt; kt < w.k1; ++kt) {
       cp_wait<STAGES - 2>();
       __syncwarp();
       {
@@ -148,7 +133,7 @@ paged_attn_few_kernel(PagedAttnArgs a) {
       }
       const uint32_t kb = smem_addr(ring + stage * STAGE), vb = kb + HALF;
       if (++stage == STAGES) stage = 0;
-      const int key0 = (kt0 + i) * TILE + warp * SLICE;
+      const int key0 = kt * TILE + warp * SLICE;
       float s[MT][2][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -203,11 +188,10 @@ paged_attn_few_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) { mma(o[m][n], pf[m], b[0], b[1]); mma(o[m][n + 1], pf[m], b[2], b[3]); }
       }
-      w.step(a, run.end);
     }
     // ---- the four warps' parts: maxima and sums first, then the outputs one warp after the other (a fixed order)
-    const bool whole = kt0 == 0 && n_tiles == tiles;
-    float *slot = whole ? nullptr : paged_slot(a, c, kt0 == 0);
+    const bool whole = w.whole();
+    float *slot = whole ? nullptr : paged_slot(a, c, pl.kt == 0);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -286,7 +270,7 @@ bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t l
 
 int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G) {
   const bool two = (long long)a.b.max_q * G > 16;
-  a.plan = paged::Plan{G, 0, two ? 32 : 16, TILE, 0, two ? PAGED_FEW_ROWS : 16};
+  a.plan = paged::Plan{G, 0, two ? 32 : 16, TILE, 2, 0, two ? PAGED_FEW_ROWS : 16};
   a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.columns = 0;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);
   return two ? launch_t<64, 2>(ctx, a) : launch_t<64, 1>(ctx, a);

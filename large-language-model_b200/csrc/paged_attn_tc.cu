@@ -42,15 +42,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // What a CTA does of one block: key tiles [k0, k1) of the block's `tiles`; tile X of its rows takes part in those below n[X].
 struct Segment {
-  int k0, k1, tiles, n[2];
-  __device__ __forceinline__ Segment(const PagedAttnArgs &a, const paged::Place &pl, long long left) {
-    const int half = a.plan.tokens_per_block / 2, t0 = pl.block * a.plan.tokens_per_block;
-    tiles = a.plan.tiles(pl.q, pl.block);
-    k0 = pl.kt; k1 = (int)min((long long)tiles, k0 + left);
+  int k0, k1, n[2];
+  __device__ __forceinline__ Segment(const PagedAttnArgs &a, const paged::Walk &w) {
+    const int half = a.plan.tokens_per_block / 2, t0 = w.pl.block * a.plan.tokens_per_block;
+    k0 = w.pl.kt; k1 = w.k1;
 #pragma unroll
     for (int X = 0; X < 2; ++X) {
-      const int first = t0 + X * half, last = min(pl.q.ql, first + half);          // tokens [first, last)
-      n[X] = first < pl.q.ql ? max(1, (min(max(pl.q.base + last, 0), pl.q.len) + TK - 1) / TK) : 0;
+      const int first = t0 + X * half, last = min(w.pl.q.ql, first + half);          // tokens [first, last)
+      n[X] = first < w.pl.q.ql ? max(1, (min(max(w.pl.q.base + last, 0), w.pl.q.len) + TK - 1) / TK) : 0;
     }
   }
   __device__ __forceinline__ int end(int X) const { return max(k0, min(k1, n[X])); }
@@ -80,6 +79,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   pdl_wait();
   pdl_launch_dependents();                       // behind the wait: the join may read the batch as soon as it starts
   const paged::Run run = paged::line_run<TC_THREADS>(a.b, a.plan, blockIdx.x, a.n_cta, a.min_units, sh->red, &sh->place);
+  if (threadIdx.x == 0) paged_write_head(a, run, sh->place, blockIdx.x);
   if (run.u == run.end) return;
   if (threadIdx.x == 0) {
     tc::mbar_init(&sh->q_full, 1); tc::mbar_init(&sh->q_empty, 1);
@@ -98,9 +98,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem_base = sh->tmem_base;
-  paged::Place pl = sh->place;
-  long long u = run.u;
   const long long end = run.end;
+  paged::Walk w;
+  w.start(a.plan, sh->place, end);
+  paged::Place &pl = w.pl;
   int seg = 0;                                   // segments so far
   bool ok = true;
 
@@ -110,8 +111,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const int half = a.plan.tokens_per_block / 2, boxes = TK / box_rows;
       const uint32_t q_bytes = (uint32_t)(half * a.plan.G * HD * 2);
       int it = 0;                                // key tiles so far
-      for (; u < end && ok; ++seg) {
-        const Segment g(a, pl, end - u);
+      for (; w.more && ok; ++seg) {
+        const Segment g(a, w);
         if (lane == 0 && seg > 0) ok = tc::mbar_wait(&sh->q_empty, (seg - 1) & 1, status, abort_flag, 261);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -159,8 +160,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (lane == 0 && j == ragged) tc::mbar_arrive(&sh->fix_ask[s]);
           page = next;
         }
-        u += g.k1 - g.k0;
-        if (u < end) paged::line_next(a.b, a.plan, pl);
+        w.next(a.b, a.plan, end);
       }
       if (*abort_flag) { long long t0 = clock64(); while (clock64() - t0 < 2000000ll) {} }      // copies in flight land before the CTA ends
     } else if (warp == MMA_WARP) {
@@ -169,8 +169,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         constexpr uint32_t idesc_o = tc::make_idesc_bf16(128, HD, false, true);
         const uint32_t q_addr[2] = {tc::smem_u32(sQ), tc::smem_u32(sQ + TILE_BYTES)};
         int it = 0, fixes[2] = {0, 0}, done[2] = {0, 0};  // done[X]: products with V issued for row tile X; fixes: per buffer
-        for (; u < end && ok; ++seg) {
-          const Segment g(a, pl, end - u);
+        for (; w.more && ok; ++seg) {
+          const Segment g(a, w);
           const int e[2] = {g.end(0), g.end(1)}, last_X = g.n[1] ? 1 : 0, ragged = g.ragged(pl);
           bool fixed = false;
           ok = tc::mbar_wait(&sh->q_full, seg & 1, status, abort_flag, 264);
@@ -215,16 +215,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             if (ok && j < e[1]) { ok = issue_pv(1, j); if (ok && j + 1 < e[1]) ok = issue_s(1, j + 1); }
           }
           it += g.k1 - g.k0;
-          u += g.k1 - g.k0;
-          if (u < end) paged::line_next(a.b, a.plan, pl);
+          w.next(a.b, a.plan, end);
         }
       }
     } else if (warp == FIX_WARP) {
       // The load warp asks, per buffer, once the tile's copy is under way: a buffer is not loaded again before its repair was used, so
       // neither side of these barriers, nor the full barrier waited for here, can be more than one phase away.
       int it = 0, fixes[2] = {0, 0};
-      while (u < end && ok) {
-        const Segment g(a, pl, end - u);
+      while (w.more && ok) {
+        const Segment g(a, w);
         const int j = g.ragged(pl);
         if (j >= 0) {
           const int i = it + j - g.k0, s = i & 1;
@@ -243,8 +242,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (lane == 0) tc::mbar_arrive(&sh->fix_done[s]);
         }
         it += g.k1 - g.k0;
-        u += g.k1 - g.k0;
-        if (u < end) paged::line_next(a.b, a.plan, pl);
+        w.next(a.b, a.plan, end);
       }
     }
   } else {
@@ -254,8 +252,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const float sl2 = a.scale * PAGED_LOG2E;
     const uint32_t tS = tmem_base + ((uint32_t)(quarter * 32) << 16) + X * 256, tO = tS + 128;
     int cnt = 0;                                           // tiles of this row tile so far
-    while (u < end && ok) {
-      const Segment g(a, pl, end - u);
+    while (w.more && ok) {
+      const Segment g(a, w);
       const int jx = g.end(X);
       int row, head, pos;
       const bool has = paged_row(a, pl, r, row, head, pos);
@@ -310,15 +308,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         // probabilities, rounded to bf16 for the tensor product, over the first half of the score columns (all 128 were read above)
         float rs4[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[64];
+        uint32_t pk[64];
 #pragma unroll
         for (int i = 0; i < 128; i += 2) {
           const float e0 = fast_exp2(__uint_as_float(v[i]) * sl2 - m_used), e1 = fast_exp2(__uint_as_float(v[i + 1]) * sl2 - m_used);
           rs4[(i >> 1) & 3] += e0 + e1;
-          w[i >> 1] = pack_bf16(e0, e1);
+          pk[i >> 1] = pack_bf16(e0, e1);
         }
-        tc::tmem_st_32x32(tS, w);
-        tc::tmem_st_32x32(tS + 32, w + 32);
+        tc::tmem_st_32x32(tS, pk);
+        tc::tmem_st_32x32(tS + 32, pk + 32);
         l += (rs4[0] + rs4[1]) + (rs4[2] + rs4[3]);
         tc::tmem_st_wait();
         tc::tc_fence_before();
@@ -327,7 +325,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       if (!ok) break;
       // ---- the block's end, or the run's: normalised rows, or a partial result
-      const bool whole = g.k0 == 0 && g.k1 == g.tiles, any = jx > g.k0;
+      const bool whole = w.whole(), any = jx > g.k0;
       if (any) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh->o_full[X], (cnt - 1) & 1, status, abort_flag, 272));
         if (!ok) break;
@@ -381,8 +379,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
       }
       tc::tc_fence_before();
-      u += g.k1 - g.k0;
-      if (u < end) paged::line_next(a.b, a.plan, pl);
+      w.next(a.b, a.plan, end);
     }
   }
   tc::tc_fence_before();
@@ -427,7 +424,7 @@ bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const vo
 }
 
 int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs a, int G, int min_rows) {
-  a.plan = paged::Plan{G, 2 * (128 / G), 0, TK, min_rows, 0x7fffffff};
+  a.plan = paged::Plan{G, 2 * (128 / G), 0, TK, 1, min_rows, 0x7fffffff};
   a.n_cta = ctx->sm_count; a.min_units = 2; a.slot_rows = 256; a.columns = 1;
   return a.b.hd == 128 ? launch_t<128>(ctx, a) : launch_t<64>(ctx, a);
 }

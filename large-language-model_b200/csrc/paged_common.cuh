@@ -68,12 +68,13 @@ __host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int p
 
 // ---- division of the work ---------------------------------------------------------------------------------------------
 // A sequence's rows (token, query head of the group) are cut into blocks; a block walks the key tiles its last row can see.
-// All (sequence, KV head, block, tile) in this order form one line of `total` units, and CTA c of n works on
-// [c * total / n, (c + 1) * total / n): every SM gets the same number of tiles whatever the lengths are.  A block that
-// crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
+// All (sequence, KV head, block, tile) in this order form one line; a block takes `extra` units (its start and end, in tiles' time)
+// and one per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
+// whatever the lengths are (without the extra, CTAs whose run held dozens of short sequences took 1.8 times the others' time).
+// A block that crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
 struct Plan {
   int G, tokens_per_block, rows_per_block;   // rows_per_block > 0: blocks of consecutive rows; else blocks of whole tokens
-  int tile, min_rows, max_rows;              // keys per tile; only sequences with min_rows <= rows <= max_rows take part
+  int tile, extra, min_rows, max_rows;       // keys per tile; only sequences with min_rows <= rows <= max_rows take part
   __host__ __device__ __forceinline__ bool takes(int ql) const { const long long r = (long long)ql * G; return ql > 0 && r >= min_rows && r <= max_rows; }
   __host__ __device__ __forceinline__ int blocks(int ql) const {
     return rows_per_block ? (int)(((long long)ql * G + rows_per_block - 1) / rows_per_block) : (ql + tokens_per_block - 1) / tokens_per_block;
@@ -85,24 +86,25 @@ struct Plan {
     return greater(1, (seen + tile - 1) / tile);   // a block that sees nothing still writes its empty rows
   }
 };
-struct Place { int seq, kvh, block, kt; Seq q; };   // a position on the line: tile kt of a block
+struct Place { int seq, kvh, block, kt; Seq q; long long first; };   // tile kt of a block, which begins at unit `first`
 
 __host__ __device__ __forceinline__ long long seq_units(const PagedArgs &a, const Plan &p, int s) {
   const Seq q = load_seq(a, s);
   if (!p.takes(q.ql)) return 0;
   long long u = 0;
-  for (int b = p.blocks(q.ql) - 1; b >= 0; --b) u += p.tiles(q, b);
+  for (int b = p.blocks(q.ql) - 1; b >= 0; --b) u += p.tiles(q, b) + p.extra;
   return u * a.n_kv;
 }
 
-// Unit `rest` of sequence s, which has `units`.
-__host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Plan &p, int s, long long units, long long rest) {
+// Unit u of the line, which is in sequence s, whose units begin at `at` and number `units`.
+__host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Plan &p, int s, long long units, long long at, long long u) {
   const long long per_head = units / a.n_kv;
   Place pl;
-  pl.seq = s; pl.q = load_seq(a, s); pl.kvh = (int)(rest / per_head); rest -= pl.kvh * per_head;
-  int b = 0, t = p.tiles(pl.q, 0);
-  while (rest >= t) { rest -= t; t = p.tiles(pl.q, ++b); }
-  pl.block = b; pl.kt = (int)rest;
+  pl.seq = s; pl.q = load_seq(a, s); pl.kvh = (int)((u - at) / per_head);
+  pl.first = at + pl.kvh * per_head;
+  int b = 0, t = p.tiles(pl.q, 0) + p.extra;
+  while (u - pl.first >= t) { pl.first += t; t = p.tiles(pl.q, ++b) + p.extra; }
+  pl.block = b; pl.kt = greater(0, (int)(u - pl.first) - p.extra);
   return pl;
 }
 
@@ -145,7 +147,7 @@ __device__ Run line_run(const PagedArgs &a, const Plan &p, int c, int n_max, int
   if (total == 0 || c >= r.n) return r;
   r.u = line_at(total, r.n, c); r.end = line_at(total, r.n, c + 1);
   if (a.n_seq <= THREADS) {                                // each thread has one sequence: the scan above is the line
-    if (r.u >= at && r.u < at + mine) *out = place_in(a, p, tid, mine, r.u - at);
+    if (r.u >= at && r.u < at + mine) *out = place_in(a, p, tid, mine, at, r.u);
   } else {
     long long done = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += THREADS) {
@@ -153,7 +155,7 @@ __device__ Run line_run(const PagedArgs &a, const Plan &p, int c, int n_max, int
       const long long m = s0 == 0 ? first : s < a.n_seq ? seq_units(a, p, s) : 0;
       long long sum;
       at = done + block_scan<THREADS>(m, red, sum);
-      if (r.u >= at && r.u < at + m) *out = place_in(a, p, s, m, r.u - at);
+      if (r.u >= at && r.u < at + m) *out = place_in(a, p, s, m, at, r.u);
       done += sum;
       if (done > r.u) break;                               // the same for all threads
     }
@@ -161,17 +163,42 @@ __device__ Run line_run(const PagedArgs &a, const Plan &p, int c, int n_max, int
   __syncthreads();
   return r;
 }
-// The start of the next block on the line.
-__host__ __device__ __forceinline__ void line_next(const PagedArgs &a, const Plan &p, Place &pl) {
-  pl.kt = 0;
-  if (++pl.block < p.blocks(pl.q.ql)) return;
-  pl.block = 0;
-  if (++pl.kvh < a.n_kv) return;
-  pl.kvh = 0;
-  while (++pl.seq < a.n_seq) {
-    pl.q = load_seq(a, pl.seq);
-    if (p.takes(pl.q.ql)) return;
+// Steps through a run block by block: tiles [pl.kt, k1) of the block's `tiles`.
+struct Walk {
+  Place pl;
+  int tiles, k1;
+  bool more;
+  __host__ __device__ __forceinline__ void start(const Plan &p, const Place &at, long long end) { pl = at; set(p, end); }
+  __host__ __device__ __forceinline__ void set(const Plan &p, long long end) {
+    tiles = p.tiles(pl.q, pl.block);
+    const long long room = end - pl.first - p.extra;
+    k1 = room < tiles ? (int)room : tiles;
+    more = k1 > pl.kt;                                     // a run that ends in a block's extra leaves it to the next CTA
   }
+  __host__ __device__ __forceinline__ bool whole() const { return pl.kt == 0 && k1 == tiles; }
+  __host__ __device__ __forceinline__ void next(const PagedArgs &a, const Plan &p, long long end) {
+    pl.first += tiles + p.extra;
+    pl.kt = 0;
+    if (pl.first >= end) { more = false; return; }
+    if (++pl.block >= p.blocks(pl.q.ql)) {
+      pl.block = 0;
+      if (++pl.kvh >= a.n_kv) {
+        pl.kvh = 0;
+        while (++pl.seq < a.n_seq) {
+          pl.q = load_seq(a, pl.seq);
+          if (p.takes(pl.q.ql)) break;
+        }
+        if (pl.seq >= a.n_seq) { more = false; return; }
+      }
+    }
+    set(p, end);
+  }
+};
+// How many CTAs, from c - 1 on, have parts of the block that run c begins in; 0 unless c is the first border inside that block.
+__host__ __device__ __forceinline__ int parts_at(const Plan &p, const Run &r, const Place &pl, int c) {
+  if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) > pl.first + p.extra) return 0;
+  const long long last = pl.first + p.extra + p.tiles(pl.q, pl.block), c1 = (last * r.n - 1) / r.total;      // line_at(c1) < last
+  return (int)(c1 < r.n - 1 ? c1 : r.n - 1) - c + 2;
 }
 
 }  // namespace paged
