@@ -27,9 +27,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, PER = BINS / THREADS, LIST = 512, SMALL = 256, MAX_CLUSTER = 8;
-static_assert(LIST <= THREADS && PER == 4, "one list entry and one 16-byte vector of bins a thread");
-constexpr float RANGE = 32.0f;            // in units of the temperature: below max - 32 T a weight is under half of 2^-44
+constexpr int THREADS = 1024, WARPS = THREADS / 32, BINS = 2048, PER = BINS / THREADS, LIST = 512, SMALL = 256, HELD = 2048, CHUNK = 128, MAX_CLUSTER = 8;
+static_assert(LIST <= THREADS && PER % 2 == 0, "one list entry and pairs of bins a thread");
+constexpr float RANGE = 32.0f;            // in units of the temperature: from max - 32 T on a weight is under a quarter of 2^-44
 typedef unsigned long long u64;
 
 struct GivenArgs {
@@ -46,16 +46,17 @@ struct alignas(16) Entry { uint32_t key, id; u64 q; };
 struct alignas(16) Mail { u64 a, b; };
 struct Found { u64 above_c, above_m, cnt, mass; int bin; };
 struct alignas(16) Shared {
-  uint32_t cnt[BINS], lo[BINS], hi[BINS];    // this CTA's histogram; a bin's weight is hi : lo
+  uint32_t coarse[BINS];                     // this CTA's counts below the maximum
+  uint32_t cnt[BINS], lo[BINS], hi[BINS];    // its finer histogram; a bin's weight is hi : lo
   Entry list[LIST];
+  uint2 held[HELD];                          // (key, id) of the ids between the bounds of top-p's border
   double table[64];                          // 2^(j / 64)
   Mail mail[2][MAX_CLUSTER];
-  Mail warp_mail[MAX_CLUSTER * WARPS];
-  uint32_t warp_eq[MAX_CLUSTER * WARPS];
-  u64 red[WARPS], red2[WARPS], sums[2], res[4];
+  u64 red[WARPS], red2[WARPS], res[4];
   Found found;
-  int bounds[2];
-  int list_n;
+  int bounds[2], list_n, held_n, pick_chunk;
+  uint32_t last_id;
+  u64 pick_before;
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t b = __float_as_uint(x); return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
@@ -63,14 +64,14 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 // -0 is 0; NaN counts as masked
 __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
 
-// exp(z) for z2 = z / ln 2 <= 0: 2^(k/64) from a table times a polynomial of the rest (|rest| <= 2^-7, degree 5: error 3e-17).
+// 2^z2 for z2 in [-1020, 0]: 2^(k/64) from a table times the exponential series in (rest ln 2), |rest| <= 2^-7, to degree 5 (error 3e-17).
 __device__ __forceinline__ double weight(double z2, const double *table) {
-  if (!(z2 > -1020.0)) return 0.0;
+  constexpr double L = 0.69314718055994530942, L2 = L * L, L3 = L2 * L, L4 = L3 * L, L5 = L4 * L;
   const double shift = 6755399441055744.0;      // 1.5 * 2^52: adding it rounds to an integer held in the low bits
-  const double t = z2 * 64.0 + shift;
+  const double t = fma(z2, 64.0, shift);
   const int k = __double2loint(t);
-  const double r = (z2 - (t - shift) * 0.015625) * 0.69314718055994530942;
-  const double p = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0);
+  const double r = fma(t - shift, -0.015625, z2);
+  const double p = fma(r, fma(r, fma(r, fma(r, fma(r, L5 / 120, L4 / 24), L3 / 6), L2 / 2), L), 1.0);
   const double m = p * table[k & 63];           // in (0.99, 2.01)
   return __hiloint2double(__double2hiint(m) + ((k >> 6) << 20), __double2loint(m));
 }
@@ -85,40 +86,37 @@ __device__ __forceinline__ u64 block_add(u64 v, u64 *red) {
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  u64 t = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) t += red[i];
-  return t;
+  return warp_add((threadIdx.x & 31) < WARPS ? red[threadIdx.x & 31] : 0ull);
 }
 __device__ __forceinline__ void block_max2(uint32_t &a, uint32_t &b, u64 *red) {
   a = __reduce_max_sync(0xffffffffu, a); b = __reduce_max_sync(0xffffffffu, b);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ((u64)a << 32) | b;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) { a = max(a, (uint32_t)(red[i] >> 32)); b = max(b, (uint32_t)red[i]); }
+  const u64 v = (threadIdx.x & 31) < WARPS ? red[threadIdx.x & 31] : 0ull;
+  a = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32)); b = __reduce_max_sync(0xffffffffu, (uint32_t)v);
 }
 // exclusive prefixes over the threads, and the totals, of two values
 template <class V>
 __device__ __forceinline__ void block_scan2(V &a, V &b, V &sum_a, V &sum_b, V *red, V *red2) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  V ia = a, ib = b;
+  auto scan = [&](V &x, V &y) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const V ta = __shfl_up_sync(0xffffffffu, ia, o), tb = __shfl_up_sync(0xffffffffu, ib, o);
-    if (lane >= o) { ia += ta; ib += tb; }
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const V tx = __shfl_up_sync(0xffffffffu, x, o), ty = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) { x += tx; y += ty; }
+    }
+  };
+  V ia = a, ib = b;
+  scan(ia, ib);
   __syncthreads();
   if (lane == 31) { red[warp] = ia; red2[warp] = ib; }
   __syncthreads();
-  V before_a = 0, before_b = 0;
-  sum_a = sum_b = 0;
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    if (i < warp) { before_a += red[i]; before_b += red2[i]; }
-    sum_a += red[i]; sum_b += red2[i];
-  }
-  a = before_a + ia - a; b = before_b + ib - b;
+  V wa = lane < WARPS ? red[lane] : V(0), wb = lane < WARPS ? red2[lane] : V(0);
+  scan(wa, wb);
+  sum_a = __shfl_sync(0xffffffffu, wa, 31); sum_b = __shfl_sync(0xffffffffu, wb, 31);
+  const V pa = __shfl_sync(0xffffffffu, wa, max(warp - 1, 0)), pb = __shfl_sync(0xffffffffu, wb, max(warp - 1, 0));
+  a = (warp ? pa : V(0)) + ia - a; b = (warp ? pb : V(0)) + ib - b;
 }
 
 // The CTAs of a row.
@@ -137,7 +135,7 @@ struct Group {
   }
 };
 
-struct Border { uint32_t key; u64 ties, equal, mass; };   // least kept value; kept ids of it, all ids of it; weight of the kept prefix
+struct Border { uint32_t key, last_id; };   // least kept value, and the last id of it that is kept
 
 template <class T, int C>
 struct Row {
@@ -145,37 +143,70 @@ struct Row {
   Shared *s;
   const T *x;          // this CTA's slice
   int n, id0;          // ids in the slice, first id
-  float mx, far, scale;   // far: values below mx - far have weight 0; scale: bins per unit of the logits
-  double z_scale, one;    // log2(e) / T; the weight 1 in fixed point
+  float mx, low, scale;   // low = mx - 32 T: ids above it need no look at how small their weight is; scale: bins per unit of the logits
+  double mxd, z_scale, one;    // mx; log2(e) / T; the weight 1 in fixed point
+  bool inf_max, dirty;    // the maximum is infinite: only the ids that reach it count; values not cleaned yet
 
-  __device__ __forceinline__ double w_of(float v) const { return v == mx ? 1.0 : weight(((double)v - (double)mx) * z_scale, s->table); }
-  // exp(..) > 0 in 64 bits; weight() gives 0 from 2^-1020 on, which no sum and no min_p (a 32-bit number) can tell from 0
-  __device__ __forceinline__ bool positive(float v) const { return v == mx || ((double)v - (double)mx) * z_scale > -1075.0; }
-  __device__ __forceinline__ u64 q_of(double w) const { return (u64)(w * one + 0.5); }
-  __device__ __forceinline__ u64 q_at(float v) const { return v == mx || mx - v < far ? q_of(w_of(v)) : 0; }
+  __device__ __forceinline__ double z2_of(float v) const { return ((double)v - mxd) * z_scale; }
+  // in 64 bits; weights below 2^-1020, which no sum and no min_p (a 32-bit number) can tell from 0, are 0
+  __device__ __forceinline__ double w_of(float v) const { const double z2 = z2_of(v); return z2 > -1020.0 ? weight(z2, s->table) : 0.0; }
+  __device__ __forceinline__ bool positive(float v) const { return v > low || z2_of(v) > -1075.0; }      // exp(..) > 0 in 64 bits
+  // the weight as a whole multiple of 2^-fixed_bits: rounded next to 2^52, so the low bits of that sum are it.  What lies below 2^-46.5, masked
+  // ids among it, is taken as that, which rounds to 0.
+  __device__ __forceinline__ double at_2_52(float v) const { return fma(weight(fmax(z2_of(v), -46.5), s->table), one, 4503599627370496.0); }
+  __device__ __forceinline__ double qd_at(float v) const { return at_2_52(v) - 4503599627370496.0; }
+  __device__ __forceinline__ u64 q_at(float v) const { return (u64)(__double_as_longlong(at_2_52(v)) - 0x4330000000000000ll); }
   // distance from the maximum in bins; what lies behind the last bin is in it
-  __device__ __forceinline__ float t_of(float v) const { const float t = v == mx ? 0.f : (mx - v) * scale; return t < (float)(BINS - 1) ? t : (float)(BINS - 1); }
+  __device__ __forceinline__ float t_of(float v) const { return fminf((mx - v) * scale, (float)(BINS - 1)); }
 
-  // f(value, index in the slice) for every id
-  template <class F> __device__ __forceinline__ void each(F f) const {
-    constexpr int N = 16 / sizeof(T);
-    if (((uintptr_t)x & 15) == 0) {
-      const int nv = n / N;
-      for (int i = threadIdx.x; i < nv; i += THREADS) {
-        Vec16<T> v;
-        float e[N];
-        v.load(x + i * N); v.unpack(e);
-#pragma unroll
-        for (int j = 0; j < N; ++j) f(clean(e[j]), i * N + j);
+  // ids i .. i + 3 of the slice, -inf from `end` on; i is a multiple of four
+  __device__ __forceinline__ void load4(int i, int end, float (&e)[4]) const {
+    if (i + 4 <= end && ((uintptr_t)x & (4 * sizeof(T) - 1)) == 0) {
+      if constexpr (sizeof(T) == 4) { const float4 v = *reinterpret_cast<const float4 *>(x + i); e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w; }
+      else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(x + i);
+        e[0] = __uint_as_float(v.x << 16); e[1] = __uint_as_float(v.x & 0xffff0000u); e[2] = __uint_as_float(v.y << 16); e[3] = __uint_as_float(v.y & 0xffff0000u);
       }
-      for (int i = nv * N + threadIdx.x; i < n; i += THREADS) f(clean(to_f(x[i])), i);
     } else {
-      for (int i = threadIdx.x; i < n; i += THREADS) f(clean(to_f(x[i])), i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = i + j < end ? to_f(x[i + j]) : -INFINITY;
+    }
+    if (dirty) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = clean(e[j]);
+    }
+    if (inf_max) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = e[j] == INFINITY ? 0.f : -INFINITY;
     }
   }
+  __device__ __forceinline__ float one_of(int i, int end) const {
+    const float v = i < end ? clean(to_f(x[i])) : -INFINITY;
+    return !inf_max ? v : v == INFINITY ? 0.f : -INFINITY;
+  }
+  // f(values, index of the first in the slice): four consecutive ids at a time
+  template <class F> __device__ __forceinline__ void each4(F f) const {
+    for (int i = threadIdx.x * 4; i < n; i += THREADS * 4) {
+      float e[4];
+      load4(i, n, e);
+      f(e, i);
+    }
+  }
+  // f(value, index in the slice) for every finite id of at least `least`
+  template <class F> __device__ __forceinline__ void each(float least, F f) const {
+    each4([&](const float (&e)[4], int i) {
+      if (!(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= least)) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) if (e[j] >= least && e[j] > -INFINITY) f(e[j], i + j);
+    });
+  }
+  // a value below every id of bins 0 .. bin
+  __device__ __forceinline__ float below(int bin) const {
+    if (bin >= BINS - 1 || !(scale > 0.f)) return -INFINITY;
+    return mx - (float)(bin + 2) / scale;
+  }
   __device__ __forceinline__ void clear() {
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    reinterpret_cast<uint4 *>(s->cnt)[threadIdx.x] = z; reinterpret_cast<uint4 *>(s->lo)[threadIdx.x] = z; reinterpret_cast<uint4 *>(s->hi)[threadIdx.x] = z;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) s->cnt[i] = s->lo[i] = s->hi[i] = 0;
   }
   __device__ __forceinline__ void add(int bin, u64 q) {
     atomicAdd(&s->cnt[bin], 1u);
@@ -185,23 +216,27 @@ struct Row {
     if (h) atomicAdd(&s->hi[bin], h);
   }
   // The cluster's sums of this thread's PER bins (call after a sync; the histograms must stay until the next one).
-  __device__ __forceinline__ void counts(u64 (&c)[PER]) {
+  __device__ __forceinline__ void counts(uint32_t *from, u64 (&c)[PER]) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) c[j] = 0;
 #pragma unroll
-    for (int r = 0; r < C; ++r) {
-      const uint4 v = reinterpret_cast<const uint4 *>(g.peer(s->cnt, r))[threadIdx.x];
-      c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
-    }
+    for (int r = 0; r < C; ++r)
+#pragma unroll
+      for (int j = 0; j < PER; j += 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(g.peer(from, r) + threadIdx.x * PER + j);
+        c[j] += v.x; c[j + 1] += v.y;
+      }
   }
   __device__ __forceinline__ void weights(u64 (&m)[PER]) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) m[j] = 0;
 #pragma unroll
-    for (int r = 0; r < C; ++r) {
-      const uint4 l = reinterpret_cast<const uint4 *>(g.peer(s->lo, r))[threadIdx.x], h = reinterpret_cast<const uint4 *>(g.peer(s->hi, r))[threadIdx.x];
-      m[0] += ((u64)h.x << 32) + l.x; m[1] += ((u64)h.y << 32) + l.y; m[2] += ((u64)h.z << 32) + l.z; m[3] += ((u64)h.w << 32) + l.w;
-    }
+    for (int r = 0; r < C; ++r)
+#pragma unroll
+      for (int j = 0; j < PER; j += 2) {
+        const uint2 l = *reinterpret_cast<const uint2 *>(g.peer(s->lo, r) + threadIdx.x * PER + j), h = *reinterpret_cast<const uint2 *>(g.peer(s->hi, r) + threadIdx.x * PER + j);
+        m[j] += ((u64)h.x << 32) + l.x; m[j + 1] += ((u64)h.y << 32) + l.y;
+      }
   }
   // The bin where the running total from the top reaches the target: above < target <= above + bin.  Every CTA finds it for itself.
   __device__ Found search(const u64 (&c)[PER], const u64 (&m)[PER], bool by_mass, double target, u64 start_c, u64 start_m) {
@@ -222,66 +257,96 @@ struct Row {
     return f;
   }
 
-  // Sends the ids that `member` selects to the first CTA's list; returns after the list is complete.
-  template <class M> __device__ __forceinline__ void gather(M member) {
+  // Sends the ids that `member` selects to the first CTA's list; returns after the list is complete.  From the held ids where `held`.
+  template <class M> __device__ __forceinline__ void gather(float least, bool held, M member) {
     Shared *first = g.peer(s, 0);
-    each([&](float v, int i) {
-      const uint32_t k = key_of(v);
-      if (v > -INFINITY && member(v, k)) {
-        const int at = atomicAdd(&first->list_n, 1);
-        if (at < LIST) *reinterpret_cast<uint2 *>(&first->list[at]) = make_uint2(k, (uint32_t)(id0 + i));
-      }
-    });
+    auto send = [&](uint32_t k, uint32_t id) {
+      const int at = atomicAdd(&first->list_n, 1);
+      if (at < LIST) *reinterpret_cast<uint2 *>(&first->list[at]) = make_uint2(k, id);
+    };
+    if (held) {
+      for (int i = threadIdx.x; i < s->held_n; i += THREADS) { const uint2 h = s->held[i]; if (member(value_of(h.x), h.x)) send(h.x, h.y); }
+    } else {
+      each(least, [&](float v, int i) { const uint32_t k = key_of(v); if (member(v, k)) send(k, (uint32_t)(id0 + i)); });
+    }
     g.sync();
   }
   // The first CTA: each entry's weight, then the ids and the weight ahead of this thread's entry in the order.  All its threads call.
-  __device__ __forceinline__ int rank_list(Entry &e, u64 &ahead_c, u64 &ahead_m, u64 &eq_ahead, u64 &equal) {
+  __device__ __forceinline__ int rank_list(Entry &e, u64 &ahead_c, u64 &ahead_m) {
     const int n_list = min(s->list_n, LIST), i = threadIdx.x;
     e = Entry{0, 0, 0};
     if (i < n_list) { e = s->list[i]; e.q = q_at(value_of(e.key)); s->list[i].q = e.q; }
     __syncthreads();
-    ahead_c = ahead_m = eq_ahead = equal = 0;
+    ahead_c = ahead_m = 0;
     if (i < n_list) {
-      uint32_t c = 0, q = 0, eq = 0;
+      uint32_t c = 0;
 #pragma unroll 4
       for (int j = 0; j < n_list; ++j) {
         const Entry o = s->list[j];
-        const bool same = o.key == e.key, ahead = o.key > e.key || (same && o.id < e.id);
-        c += ahead; q += same && ahead; eq += same;
+        const bool ahead = o.key > e.key || (o.key == e.key && o.id < e.id);
+        c += ahead;
         ahead_m += ahead ? o.q : 0;
       }
-      ahead_c = c; eq_ahead = q; equal = eq;
+      ahead_c = c;
     }
     return n_list;
   }
 
-  // Settles the border inside a bin.  `member(value, key)` selects the bin's ids; the list must be empty (and is again afterwards).
+  // The t-th id, in id order, of those with this value.  Each warp counts a run of ids, then one walks its own.
+  __device__ uint32_t nth_equal(uint32_t key, u64 t) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, run = (n + WARPS - 1) / WARPS, i0 = min(n, warp * run), i1 = min(n, i0 + run);
+    uint32_t mine = 0;
+    for (int i = i0 + lane; i < i1; i += 32) mine += key_of(one_of(i, i1)) == key;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    u64 before = lane == 0 ? mine : 0, none = 0, sum, zero;
+    block_scan2<u64>(before, none, sum, zero, s->red, s->red2);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    const Mail *all = g.exchange(sum, 0);
+    for (int r = 0; r < g.rank; ++r) before += all[r].a;
+    if (before < t && t <= before + mine) {
+      u64 at = before;
+      for (int i = i0; i < i1; i += 32) {
+        const unsigned same = __ballot_sync(0xffffffffu, i + lane < i1 && key_of(one_of(i + lane, i1)) == key);
+        if (at + __popc(same) >= t) {
+          if ((same >> lane & 1) && at + __popc(same & ((2u << lane) - 1)) == t)
+            for (int r = 0; r < C; ++r) *g.peer(&s->last_id, r) = (uint32_t)(id0 + i + lane);
+          break;
+        }
+        at += __popc(same);
+      }
+    }
+    g.sync();
+    return s->last_id;
+  }
+
+  // Settles the border inside a bin.  `member(value, key)` selects the bin's ids, all of them at least `least` and, where `held`, among the held
+  // ones; the list must be empty (and is again afterwards).  by_k: the target is a count.
   template <class M>
-  __device__ Border settle(M member, Found f, bool by_mass, double target) {
+  __device__ Border settle(float least, bool held, M member, Found f, bool by_mass, double target) {
     bool narrowed = false;
     uint32_t kl = 0, kh = 0xffffffffu;
     for (int round = 0; round < 5; ++round) {
       if (f.cnt <= LIST) {
-        if (narrowed) gather([&](float, uint32_t k) { return k >= kl && k <= kh; });
-        else gather(member);
+        if (narrowed) gather(value_of(kl), held, [&](float, uint32_t k) { return k >= kl && k <= kh; });
+        else gather(least, held, member);
         if (g.rank == 0) {
           Entry e;
-          u64 rc, rm, eq_before, equal;
-          const int n_list = rank_list(e, rc, rm, eq_before, equal);
+          u64 rc, rm;
+          const int n_list = rank_list(e, rc, rm);
           rc += f.above_c; rm += f.above_m;
           const double lo = by_mass ? (double)rm : (double)rc, hi = by_mass ? (double)(rm + e.q) : (double)(rc + 1);
           if ((int)threadIdx.x < n_list && lo < target && target <= hi) {
 #pragma unroll
-            for (int r = 0; r < C; ++r) { u64 *o = g.peer(s->res, r); o[0] = e.key; o[1] = eq_before + 1; o[2] = equal; o[3] = rm + e.q; }
+            for (int r = 0; r < C; ++r) { u64 *o = g.peer(s->res, r); o[0] = e.key; o[1] = e.id; }
           }
           if (threadIdx.x == 0) s->list_n = 0;
         }
         g.sync();
-        return Border{(uint32_t)s->res[0], s->res[1], s->res[2], s->res[3]};
+        return Border{(uint32_t)s->res[0], (uint32_t)s->res[1]};
       }
       if (!narrowed) {                                      // the bin's range of values
         uint32_t h = 0, l = 0;                              // l holds ~key
-        each([&](float v, int) { const uint32_t k = key_of(v); if (v > -INFINITY && member(v, k)) { h = max(h, k); l = max(l, ~k); } });
+        each(least, [&](float v, int) { const uint32_t k = key_of(v); if (member(v, k)) { h = max(h, k); l = max(l, ~k); } });
         block_max2(h, l, s->red);
         const Mail *all = g.exchange(h, l);
 #pragma unroll
@@ -296,26 +361,26 @@ struct Row {
           t = q ? (u64)ceil(need / (double)q) : 1;
           t = t < 1 ? 1 : t > f.cnt ? f.cnt : t;
         } else t = (u64)target - f.above_c;
-        return Border{kl, t, f.cnt, f.above_m + t * q};
+        return Border{kl, nth_equal(kl, t)};
       }
       const int sh = max(0, 21 - __clz(kh - kl));           // (kh - kl) >> sh is below 2048
       g.sync();                                             // all have read the histograms that go now
       clear();
       __syncthreads();
-      each([&](float v, int) {
+      each(value_of(kl), [&](float v, int) {
         const uint32_t k = key_of(v);
-        if (v > -INFINITY && k >= kl && k <= kh) add((int)((kh - k) >> sh), q_at(v));
+        if (k >= kl && k <= kh) add((int)((kh - k) >> sh), q_at(v));
       });
       g.sync();
       u64 c[PER], m[PER];
-      counts(c); weights(m);
+      counts(s->cnt, c); weights(m);
       f = search(c, m, by_mass, target, f.above_c, f.above_m);
       const uint32_t top = kh - ((uint32_t)f.bin << sh);
-      const u64 low = (u64)((uint32_t)f.bin + 1) << sh;
-      kl = low > (u64)(kh - kl) ? kl : kh - (uint32_t)low + 1;
+      const u64 low_ = (u64)((uint32_t)f.bin + 1) << sh;
+      kl = low_ > (u64)(kh - kl) ? kl : kh - (uint32_t)low_ + 1;
       kh = top;
     }
-    return Border{kl, f.cnt, f.cnt, f.above_m + f.mass};    // not reached: three cuts leave one value
+    return Border{kl, 0xffffffffu};                         // not reached: three cuts leave one value
   }
 };
 
@@ -326,18 +391,20 @@ sample_given_kernel(GivenArgs a) {
   pdl_wait();
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared *s = (Shared *)dyn;
-  T *copy = (T *)(dyn + sizeof(Shared));
+  u64 *chunk = (u64 *)(dyn + sizeof(Shared));               // kept weight of each 128 ids of the slice
+  T *copy = (T *)(chunk + (a.slice + CHUNK - 1) / CHUNK + (((a.slice + CHUNK - 1) / CHUNK) & 1));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x / C;
   Row<T, C> row;
-  row.s = s; row.g.s = s; row.g.par = 0; row.one = (double)(1ll << a.fixed_bits);
+  row.s = s; row.g.s = s; row.g.par = 0; row.one = (double)(1ll << a.fixed_bits); row.inf_max = false;
   row.g.rank = C > 1 ? (int)(blockIdx.x % C) : 0;
   row.id0 = min(a.V, row.g.rank * a.slice); row.n = min(a.V, row.id0 + a.slice) - row.id0;
   row.x = (const T *)a.logits + (size_t)b * a.ld + row.id0;
-  const float T_ = a.temperature ? a.temperature[b] : 1.0f, p = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f, u_ = a.uniform[b];
+  const float T_in = a.temperature ? a.temperature[b] : 1.0f, T_ = T_in > 0x1p100f ? 0x1p100f : T_in, p = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f, u_ = a.uniform[b];
   const int k = a.top_k ? a.top_k[b] : 0;
   if (tid < 64) s->table[tid] = exp2(tid * 0.015625);
-  if (tid == 0) s->list_n = 0;
+  if (tid == 0) s->list_n = s->held_n = 0;
   row.clear();
+  for (int i = tid; i < BINS; i += THREADS) s->coarse[i] = 0;
   // ---- one read of the slice: a copy in shared memory, the largest and the smallest finite value
   uint32_t hi = 0, lo = 0;
   {
@@ -366,6 +433,7 @@ sample_given_kernel(GivenArgs a) {
     }
   }
   block_max2(hi, lo, s->red);
+  row.dirty = !a.in_smem;
   if (a.in_smem) row.x = copy;
   if (C > 1) {
     row.g.sync();                                            // every CTA of the cluster runs before its memory is written
@@ -379,10 +447,12 @@ sample_given_kernel(GivenArgs a) {
     return;
   }
   row.mx = value_of(hi);
-  const float mn = value_of(~lo);
+  float mn = value_of(~lo);
+  if (row.mx == INFINITY) { row.inf_max = true; row.mx = mn = 0.f; }
+  row.mxd = (double)row.mx;
   if (!(T_ > 0.f)) {                                         // greedy: the lowest id of the maximum
     uint32_t best = 0, none = 0;                             // ~id
-    row.each([&](float v, int i) { if (v == row.mx) best = max(best, ~(uint32_t)(row.id0 + i)); });
+    row.each(row.mx, [&](float v, int i) { if (v == row.mx) best = max(best, ~(uint32_t)(row.id0 + i)); });
     block_max2(best, none, s->red);
     const Mail *all = row.g.exchange(best, 0);
 #pragma unroll
@@ -392,26 +462,31 @@ sample_given_kernel(GivenArgs a) {
     return;
   }
   row.z_scale = 1.44269504088896340736 / (double)T_;
-  row.far = RANGE * T_;
+  row.low = row.mx - RANGE * T_;
   const bool by_k = k > 0 && k < a.V, by_p = p < 1.f;
   const double min_w = mp > 0.f ? fmin((double)mp, 1.0) : 0.0, frac = p > 0.f ? (double)p : 0.0;      // p <= 0 keeps the first id
   const double u = u_ > 0.f ? (double)fminf(u_, 0.99999994f) : 0.0;
-  // ---- the kept prefix
-  uint32_t vkey = 0;                                         // keep keys above it, and `ties` of the ids that have it
-  u64 ties = 0, equal = 0;
+  // ---- the kept prefix: values above `least`, and ids of that value up to last_id
+  float least = -INFINITY;
+  uint32_t last_id = 0xffffffffu;
+  int b0 = 0, b1 = BINS - 1, last_bin = BINS - 1;
+  bool have_k = false;
+  u64 c[PER];
   if (by_k || by_p) {
-    const float range = fminf(row.mx - mn, row.far);
+    const float range = fminf(row.mx - mn, RANGE * T_);
     row.scale = range > 0.f && range < INFINITY ? (float)(BINS - 1) / range : 0.f;
     if (!(row.scale < INFINITY)) row.scale = 0.f;            // a temperature next to 0: one bin, cut by the bits of the values
-    row.each([&](float v, int) { if (v > -INFINITY) atomicAdd(&s->cnt[(int)row.t_of(v)], 1u); });
+    row.each4([&](const float (&e)[4], int) {
+      int bin[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bin[j] = (int)row.t_of(e[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) if (e[j] > -INFINITY) atomicAdd(&s->coarse[bin[j]], 1u);
+    });
     row.g.sync();
-    u64 c[PER], zero[PER] = {0, 0, 0, 0};
-    row.counts(c);
-    bool have_k = false;
-    u64 mass_k = 0;
-    int last_bin = BINS - 1;
+    row.counts(s->coarse, c);
     if (by_k) {
-      u64 all_c = 0;
+      u64 all_c = 0, zero[PER] = {};
 #pragma unroll
       for (int j = 0; j < PER; ++j) all_c += c[j];
       if ((u64)k < block_add(all_c, s->red)) {               // else fewer ids than k: nothing to cut
@@ -420,11 +495,11 @@ sample_given_kernel(GivenArgs a) {
         have_k = true;
         if (f.above_c + f.cnt <= SMALL) {
           // few candidates: the first CTA does the rest among them
-          row.gather([&](float v, uint32_t) { return (int)row.t_of(v) <= f.bin; });
+          row.gather(row.below(f.bin), false, [&](float v, uint32_t) { return (int)row.t_of(v) <= f.bin; });
           if (row.g.rank == 0) {
             Entry e;
-            u64 rank, before, d0, d1;
-            const int n_list = row.rank_list(e, rank, before, d0, d1);
+            u64 rank, before;
+            const int n_list = row.rank_list(e, rank, before);
             const bool in_k = tid < n_list && rank < (u64)k;
             const u64 mass = block_add(in_k ? e.q : 0, s->red);
             const double w = in_k ? row.w_of(value_of(e.key)) : 0.0;
@@ -445,8 +520,9 @@ sample_given_kernel(GivenArgs a) {
           }
           return;                                            // nobody reads another CTA's memory any more
         }
-        const Border bd = row.settle([&](float v, uint32_t) { return (int)row.t_of(v) == f.bin; }, f, false, (double)k);
-        vkey = bd.key; ties = bd.ties; equal = bd.equal;
+        const Border bd = row.settle(row.below(f.bin), false, [&](float v, uint32_t) { return (int)row.t_of(v) == f.bin; }, f, false, (double)k);
+        least = value_of(bd.key); last_id = bd.last_id;
+        if (by_p && f.cnt > LIST) { row.g.sync(); row.clear(); __syncthreads(); }      // the bin was cut again: its histogram goes
       }
     }
     if (by_p) {
@@ -476,119 +552,154 @@ sample_given_kernel(GivenArgs a) {
         if (at_dn >= want_hi) first_dn = tid * PER + j;
       }
       first_up = __reduce_min_sync(0xffffffffu, first_up); first_dn = __reduce_min_sync(0xffffffffu, first_dn);
-      if (lane == 0) { atomicMin(&s->bounds[0], first_up); atomicMin(&s->bounds[1], first_dn); }
+      if (lane == 0) { if (first_up < BINS) atomicMin(&s->bounds[0], first_up); if (first_dn < BINS) atomicMin(&s->bounds[1], first_dn); }
       __syncthreads();
-      const int b0 = s->bounds[0], b1 = max(b0, s->bounds[1]);
-      const float fine = (float)(BINS / (b1 - b0 + 1));
-      auto fine_bin = [&](float v) { return min(BINS - 1, (int)((row.t_of(v) - (float)b0) * fine)); };
-      auto between = [&](float v, uint32_t key) { const int bin = (int)row.t_of(v); return bin >= b0 && bin <= b1 && key >= vkey; };
-      row.g.sync();                                          // all have read the counts
-      row.clear();
-      __syncthreads();
-      u64 above = 0, all_q = 0, above_c = 0;
-      row.each([&](float v, int) {
-        const uint32_t key = key_of(v);
-        if (!(v > -INFINITY) || key < vkey) return;
-        const int bin = (int)row.t_of(v);
-        const u64 q = row.q_at(v);
-        if (!have_k || key > vkey) all_q += q;
-        if (bin < b0) { above += q; ++above_c; }
-        else if (bin <= b1) row.add(fine_bin(v), q);
-      });
-      above = block_add(above, s->red); all_q = block_add(all_q, s->red);
-      const Mail *all = row.g.exchange(above, all_q);        // its sync also completes the histograms
-      above = all_q = 0;
-#pragma unroll
-      for (int r = 0; r < C; ++r) { above += all[r].a; all_q += all[r].b; }
-      if (have_k) all_q += ties * row.q_at(value_of(vkey));
-      const double target = fmax(frac * (double)all_q, 0.5);
-      u64 m[PER];
-      row.counts(c); row.weights(m);
-      const Found f = row.search(c, m, true, target, 0, above);
-      const Border bd = row.settle([&](float v, uint32_t key) { return between(v, key) && fine_bin(v) == f.bin; }, f, true, target);
-      vkey = bd.key; ties = bd.ties; equal = bd.equal;
+      b0 = s->bounds[0]; b1 = max(b0, s->bounds[1]);
     }
   }
-  // ---- the draw, in id order: warp w of CTA r owns a run of ids
-  constexpr int N = 16 / sizeof(T);
-  const int run = ((row.n + WARPS - 1) / WARPS + N - 1) / N * N, i0 = min(row.n, warp * run), i1 = min(row.n, i0 + run), slot = row.g.rank * WARPS + warp;
-  const bool count_eq = ties < equal;                        // only some ids of the least value are kept
-  u64 eq_before = 0;
-  if (count_eq) {
-    uint32_t c = 0;
-    for (int i = i0 + lane; i < i1; i += 32) c += key_of(clean(to_f(row.x[i]))) == vkey;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane < C) *row.g.peer(&s->warp_eq[slot], lane) = c;
-    row.g.sync();
-    for (int i = lane; i < slot; i += 32) eq_before += s->warp_eq[i];
-    eq_before = warp_add(eq_before);
-  }
-  auto weigh = [&](float v, bool keep, uint32_t &n_kept) -> u64 {
-    if (!keep) return 0;
-    const bool near = v == row.mx || row.mx - v < row.far;
-    if (min_w == 0.0 && !near) { n_kept += row.positive(v); return 0; }
-    const double w = row.w_of(v);
-    if (w < min_w) return 0;
-    n_kept += row.positive(v);
-    return near ? row.q_of(w) : 0;
-  };
-  // the weight of a kept id (0: not kept); eq counts ids of the least value before it.  32 consecutive ids per call.
-  auto ordered = [&](int i, u64 &eq, uint32_t &n_kept) -> u64 {
-    const float v = i < i1 ? clean(to_f(row.x[i])) : -INFINITY;
-    const uint32_t key = key_of(v);
-    bool keep = v > -INFINITY && key >= vkey;
-    if (count_eq) {
-      const unsigned same = __ballot_sync(0xffffffffu, v > -INFINITY && key == vkey);
-      if (key == vkey) keep = keep && eq + __popc(same & ((1u << lane) - 1)) < ties;
-      eq += __popc(same);
-    }
-    return weigh(v, keep, n_kept);
-  };
-  u64 mine = 0, eq = eq_before;
-  uint32_t n_kept = 0;
-  if (count_eq || ((uintptr_t)row.x & 15)) {
-    for (int i = i0; i < i1; i += 32) mine += ordered(i + lane, eq, n_kept);
-  } else {                                                   // every id of the least value is kept: any order
-    for (int i = i0 + lane * N; i < i1; i += 32 * N) {
-      if (i + N <= i1) {
-        Vec16<T> v;
-        float e[N];
-        v.load(row.x + i); v.unpack(e);
+  const float t0 = (float)b0, t1 = (float)(b1 + 1), fine = (float)(BINS / (b1 - b0 + 1));
+  auto between = [&](float t) { return t >= t0 && t < t1; };
+  auto fine_bin = [&](float t) { return min(BINS - 1, (int)((t - t0) * fine)); };
+  auto in_prefix = [&](float v, uint32_t id) { return v > least || (v == least && id <= last_id); };
+
+  // ---- weights, chunk by chunk of 128 ids (a warp's four a lane).  Weights are whole numbers whose sums stay below 2^53 in a thread and
+  // below 2^60 in a chunk, so sums of 64-bit floats are exact in the thread and those of integers beyond.
+  // bounded: with top-p's border still open, ids above its bounds go into the chunks and the ids between them are held and counted.
+  u64 above = 0, all_q = 0, n_kept = 0;
+  auto weigh = [&](bool bounded) {
+    double above_d = 0.0, all_d = 0.0;
+    uint32_t n_thread = 0;
+    for (int ch = warp; ch * CHUNK < row.n; ch += WARPS) {
+      const int i = ch * CHUNK + lane * 4;
+      float e[4];
+      row.load4(i, row.n, e);
+      double sum = 0.0;
+      const bool any = !(least > -INFINITY) || fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= least;
+      if (__any_sync(0xffffffffu, any)) {
+        double q[4];
+        bool hit = false;
 #pragma unroll
-        for (int j = 0; j < N; ++j) { const float y = clean(e[j]); mine += weigh(y, y > -INFINITY && key_of(y) >= vkey, n_kept); }
-      } else {
-        for (int j = i; j < i1; ++j) { const float y = clean(to_f(row.x[j])); mine += weigh(y, y > -INFINITY && key_of(y) >= vkey, n_kept); }
-      }
-    }
-  }
-  mine = warp_add(mine);
-  n_kept = __reduce_add_sync(0xffffffffu, n_kept);
-  if (lane < C) *row.g.peer(&s->warp_mail[slot], lane) = Mail{mine, n_kept};
-  row.g.sync();
-  u64 before = 0, total = 0, kept = 0;
-  for (int i = lane; i < C * WARPS; i += 32) { const Mail m = s->warp_mail[i]; if (i < slot) before += m.a; total += m.a; kept += m.b; }
-  before = warp_add(before); total = warp_add(total); kept = warp_add(kept);
-  const u64 target = (u64)(u * (double)total);               // cumulative > u * total, the cumulative whole: > its floor
-  if (before <= target && target < before + mine) {
-    eq = eq_before;
-    u64 at = before;
-    for (int i = i0; i < i1; i += 32) {
-      const u64 q = ordered(i + lane, eq, n_kept);
-      u64 inc = q;
+        for (int j = 0; j < 4; ++j) q[j] = row.qd_at(e[j]);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
-      const unsigned hit = __ballot_sync(0xffffffffu, q > 0 && at + inc > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          a.tokens[b] = row.id0 + i + lane;
-          if (a.prob) a.prob[b] = (float)((double)q / (double)total);
+        for (int j = 0; j < 4; ++j) {
+          bool keep = e[j] > -INFINITY;
+          if (least > -INFINITY) keep = keep && in_prefix(e[j], (uint32_t)(row.id0 + i + j));
+          if (!keep) q[j] = 0.0;
+          if (bounded) {
+            all_d += q[j];
+            const float t = row.t_of(e[j]);
+            hit |= keep && between(t);
+            keep = keep && t < t0;
+            above_d += keep ? q[j] : 0.0;
+          }
+          if (min_w > 0.0) keep = keep && row.w_of(e[j]) >= min_w;
+          else if (keep && e[j] <= row.low) keep = row.positive(e[j]);
+          sum += keep ? q[j] : 0.0;
+          n_thread += keep;
         }
-        break;
+        if (__any_sync(0xffffffffu, hit)) {
+          bool hold[4];
+          unsigned votes[4];
+          int n_held = 0, at = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hold[j] = hit && e[j] > -INFINITY && between(row.t_of(e[j])) && in_prefix(e[j], (uint32_t)(row.id0 + i + j));
+            votes[j] = __ballot_sync(0xffffffffu, hold[j]);
+            n_held += __popc(votes[j]);
+          }
+          if (lane == 0) at = atomicAdd(&s->held_n, n_held);               // one a warp: single ones crowd the one address (13k cycles)
+          at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (hold[j]) {
+              const int to = at + __popc(votes[j] & ((1u << lane) - 1));
+              row.add(fine_bin(row.t_of(e[j])), (u64)q[j]);
+              if (to < HELD) s->held[to] = make_uint2(key_of(e[j]), (uint32_t)(row.id0 + i + j));
+            }
+            at += __popc(votes[j]);
+          }
+        }
       }
-      at += __shfl_sync(0xffffffffu, inc, 31);
+      const u64 in_chunk = warp_add((u64)sum);
+      if (lane == 0) chunk[ch] = in_chunk;
+    }
+    above = (u64)above_d; all_q = (u64)all_d; n_kept = n_thread;
+  };
+  weigh(by_p);
+  if (by_p) {
+    above = block_add(above, s->red); all_q = block_add(all_q, s->red);
+    const bool held_all = s->held_n <= HELD;
+    const Mail *all = row.g.exchange(above | (held_all ? 0 : 1ull << 63), all_q);      // its sync also completes the histograms
+    above = all_q = 0;
+    bool held = true;                                        // every CTA holds all its ids between the bounds
+#pragma unroll
+    for (int r = 0; r < C; ++r) { above += all[r].a & ~(1ull << 63); all_q += all[r].b; held = held && !(all[r].a >> 63); }
+    const double target = fmax(frac * (double)all_q, 0.5);
+    u64 m[PER];
+    row.counts(s->cnt, c); row.weights(m);
+    const Found f = row.search(c, m, true, target, 0, above);
+    const float k_least = least;
+    const Border bd = row.settle(fmaxf(row.below(b1), k_least), held, [&](float v, uint32_t) { const float t = row.t_of(v); return v >= k_least && between(t) && fine_bin(t) == f.bin; }, f, true, target);
+    least = value_of(bd.key); last_id = bd.last_id;
+    if (held) {                                              // the held ids that stay join their chunks
+      for (int i = tid; i < s->held_n; i += THREADS) {
+        const uint2 h = s->held[i];
+        const float v = value_of(h.x);
+        if (in_prefix(v, h.y) && (min_w > 0.0 ? row.w_of(v) >= min_w : row.positive(v))) {
+          atomicAdd(&chunk[((int)h.y - row.id0) / CHUNK], row.q_at(v));
+          ++n_kept;
+        }
+      }
+    } else {
+      weigh(false);
     }
   }
-  if (slot == 0 && lane == 0 && a.kept) a.kept[b] = (int)kept;
+  // ---- the draw: the chunk, in id order, then the id in it
+  const int n_chunks = (row.n + CHUNK - 1) / CHUNK, per = (n_chunks + THREADS - 1) / THREADS;
+  n_kept = block_add(n_kept, s->red);                        // (a barrier before the chunks are read)
+  u64 mine = 0, none = 0, sum, zero;
+  for (int j = 0; j < per; ++j) if (tid * per + j < n_chunks) mine += chunk[tid * per + j];
+  u64 before = mine;
+  block_scan2<u64>(before, none, sum, zero, s->red, s->red2);
+  const Mail *all = row.g.exchange(sum, n_kept);
+  u64 total = 0, kept = 0;
+#pragma unroll
+  for (int r = 0; r < C; ++r) { if (r < row.g.rank) before += all[r].a; total += all[r].a; kept += all[r].b; }
+  if (row.g.rank == 0 && tid == 0 && a.kept) a.kept[b] = (int)kept;
+  const u64 target = (u64)(u * (double)total);               // cumulative > u * total, the cumulative whole: > its floor
+  if (tid == 0) s->pick_chunk = -1;
+  __syncthreads();
+  if (before <= target && target < before + mine) {
+    int ch = tid * per;
+    while (before + chunk[ch] <= target) before += chunk[ch++];
+    s->pick_chunk = ch; s->pick_before = before;
+  }
+  __syncthreads();
+  if (warp == 0 && s->pick_chunk >= 0) {
+    const int i = s->pick_chunk * CHUNK + lane * 4;
+    float e[4];
+    row.load4(i, row.n, e);
+    u64 q[4], own = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bool keep = e[j] > -INFINITY && (!(least > -INFINITY) || in_prefix(e[j], (uint32_t)(row.id0 + i + j)));
+      if (min_w > 0.0) keep = keep && row.w_of(e[j]) >= min_w;
+      q[j] = keep ? row.q_at(e[j]) : 0;
+      own += q[j];
+    }
+    u64 at = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += t; }
+    at += s->pick_before - own;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (at <= target && target < at + q[j]) {
+        a.tokens[b] = row.id0 + i + j;
+        if (a.prob) a.prob[b] = (float)((double)q[j] / (double)total);
+      }
+      at += q[j];
+    }
+  }
 }
 
 template <class T, int C>
@@ -623,13 +734,15 @@ extern "C" int b200_sample_given(b200_ctx *ctx, const void *logits, b200_dtype d
   a.fixed_bits = std::min(44, 62 - bits);
   // CTAs per row: as many as still run at once, one per SM (clusters of eight fit 15 times on 148 SMs, of four 32 times), not below 1024
   // ids each; more where a slice would not fit in shared memory.  At 32 x 100256 in 32 bits, clusters of eight ran in three waves (96 us).
-  const size_t es = dtype_size(dt), room = 220 * 1024 - sizeof(Shared);
-  auto fit = [&](int C) { return (size_t)(C == 2 ? ctx->sm_count : C == 4 ? ctx->sm_count - 20 : ctx->sm_count - 28); };
+  const size_t es = dtype_size(dt), room = 220 * 1024;
+  auto slice = [&](int C) { return ((vocab + C - 1) / C + 15) / 16 * 16; };
+  auto fixed = [&](int C) { const size_t n = (slice(C) + CHUNK - 1) / CHUNK; return sizeof(Shared) + 8 * (n + (n & 1)); };
+  auto at_once = [&](int C) { return (size_t)(C == 2 ? ctx->sm_count : C == 4 ? ctx->sm_count - 20 : ctx->sm_count - 28); };
   int C = 1;
-  while (C < MAX_CLUSTER && (batch * 2 * C <= fit(2 * C) || vocab * es / C > room) && vocab / C > 2048) C *= 2;
-  a.slice = (int)(((vocab + C - 1) / C + 15) / 16 * 16);
-  a.in_smem = (size_t)a.slice * es <= room;
-  const size_t smem = sizeof(Shared) + (a.in_smem ? (size_t)a.slice * es : 0);
+  while (C < MAX_CLUSTER && (batch * 2 * C <= at_once(2 * C) || fixed(C) + slice(C) * es > room) && vocab / C > 2048) C *= 2;
+  a.slice = (int)slice(C);
+  a.in_smem = fixed(C) + a.slice * es <= room;
+  const size_t smem = fixed(C) + (a.in_smem ? a.slice * es : 0);      // at most 198 KiB of it fixed (2^24 ids over eight CTAs)
   if (dt == B200_BF16) return C == 1 ? launch_t<bf16, 1>(ctx, a, batch, smem) : C == 2 ? launch_t<bf16, 2>(ctx, a, batch, smem) : C == 4 ? launch_t<bf16, 4>(ctx, a, batch, smem) : launch_t<bf16, 8>(ctx, a, batch, smem);
   return C == 1 ? launch_t<float, 1>(ctx, a, batch, smem) : C == 2 ? launch_t<float, 2>(ctx, a, batch, smem) : C == 4 ? launch_t<float, 4>(ctx, a, batch, smem) : launch_t<float, 8>(ctx, a, batch, smem);
 }
