@@ -21,6 +21,7 @@
 #include "paged_common.cuh"
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -54,6 +55,7 @@ struct alignas(16) Shared {
   Mail mail[2][MAX_CLUSTER];
   u64 red[WARPS], red2[WARPS], res[4];
   Found found;
+  float edges[2];
   int bounds[2], list_n, held_n, pick_chunk;
   uint32_t last_id;
   u64 pick_before;
@@ -157,7 +159,7 @@ struct Row {
   __device__ __forceinline__ double qd_at(float v) const { return at_2_52(v) - 4503599627370496.0; }
   __device__ __forceinline__ u64 q_at(float v) const { return (u64)(__double_as_longlong(at_2_52(v)) - 0x4330000000000000ll); }
   // distance from the maximum in bins; what lies behind the last bin is in it
-  __device__ __forceinline__ float t_of(float v) const { return fminf((mx - v) * scale, (float)(BINS - 1)); }
+  __device__ __forceinline__ float t_of(float v) const { return fminf(fmaxf((mx - v) * scale, 0.f), (float)(BINS - 1)); }
 
   // ids i .. i + 3 of the slice, -inf from `end` on; i is a multiple of four
   __device__ __forceinline__ void load4(int i, int end, float (&e)[4]) const {
@@ -200,6 +202,21 @@ struct Row {
       for (int j = 0; j < 4; ++j) if (e[j] >= least && e[j] > -INFINITY) f(e[j], i + j);
     });
   }
+  // The least finite value with t_of(value) < t, infinity where there is none.  A warp calls: 32 probes a step over the bits of the values.
+  __device__ float edge(float t) const {
+    uint32_t lo = key_of(-FLT_MAX), hi = key_of(mx);
+    if (!(t > 0.f)) return INFINITY;                       // t_of(mx) = 0
+    while (lo < hi) {
+      const uint32_t step = max(1u, (hi - lo) / 32), probe = min(lo + (threadIdx.x & 31) * step, hi);
+      const unsigned yes = __ballot_sync(0xffffffffu, t_of(value_of(probe)) < t);
+      if (yes & 1) { hi = lo; break; }
+      const int f = yes ? __ffs(yes) - 1 : 32;
+      const uint32_t below_ = min(lo + (uint32_t)(f - 1) * step, hi);
+      if (f < 32) hi = min(lo + (uint32_t)f * step, hi);
+      lo = min(below_ + 1, hi);
+    }
+    return value_of(hi);
+  }
   // a value below every id of bins 0 .. bin
   __device__ __forceinline__ float below(int bin) const {
     if (bin >= BINS - 1 || !(scale > 0.f)) return -INFINITY;
@@ -241,6 +258,7 @@ struct Row {
   // The bin where the running total from the top reaches the target: above < target <= above + bin.  Every CTA finds it for itself.
   __device__ Found search(const u64 (&c)[PER], const u64 (&m)[PER], bool by_mass, double target, u64 start_c, u64 start_m) {
     u64 bc = 0, bm = 0, sc, sm;
+    if (threadIdx.x == 0) s->found = Found{0, 0, 0, 0, 0};  // (the scan's barriers come before the one that finds it)
 #pragma unroll
     for (int j = 0; j < PER; ++j) { bc += c[j]; bm += m[j]; }
     block_scan2<u64>(bc, bm, sc, sm, s->red, s->red2);
@@ -558,80 +576,85 @@ sample_given_kernel(GivenArgs a) {
     }
   }
   const float t0 = (float)b0, t1 = (float)(b1 + 1), fine = (float)(BINS / (b1 - b0 + 1));
-  auto between = [&](float t) { return t >= t0 && t < t1; };
-  auto fine_bin = [&](float t) { return min(BINS - 1, (int)((t - t0) * fine)); };
+  auto fine_bin = [&](float v) { return min(BINS - 1, (int)((row.t_of(v) - t0) * fine)); };
   auto in_prefix = [&](float v, uint32_t id) { return v > least || (v == least && id <= last_id); };
+  // The bounds as values: ids from v_above on lie above them, those from v_from on above or between.
+  float v_above = -FLT_MAX, v_from = INFINITY;
+  if (by_p) {
+    if (warp < 2) {
+      const float v = row.edge(warp ? t1 : t0);
+      if (lane == 0) s->edges[warp] = v;
+    }
+    __syncthreads();
+    v_above = s->edges[0]; v_from = s->edges[1];
+  }
 
-  // ---- weights, chunk by chunk of 128 ids (a warp's four a lane).  Weights are whole numbers whose sums stay below 2^53 in a thread and
-  // below 2^60 in a chunk, so sums of 64-bit floats are exact in the thread and those of integers beyond.
-  // bounded: with top-p's border still open, ids above its bounds go into the chunks and the ids between them are held and counted.
+  // ---- weights, chunk by chunk of 128 ids (four a lane).  Weights are whole numbers whose sums stay below 2^53 in a thread, so sums of
+  // 64-bit floats are exact there, and those of integers beyond.  With top-p's border still open (bounded), ids above its bounds go into
+  // the chunks and the ids between them are held.
   u64 above = 0, all_q = 0, n_kept = 0;
   auto weigh = [&](bool bounded) {
     double above_d = 0.0, all_d = 0.0;
     uint32_t n_thread = 0;
+    const bool cut = least > -INFINITY, look = min_w == 0.0 && !(v_above > row.low);      // look: some weights may be 0 in 64 bits
     for (int ch = warp; ch * CHUNK < row.n; ch += WARPS) {
       const int i = ch * CHUNK + lane * 4;
       float e[4];
       row.load4(i, row.n, e);
-      double sum = 0.0;
-      const bool any = !(least > -INFINITY) || fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) >= least;
-      if (__any_sync(0xffffffffu, any)) {
-        double q[4];
-        bool hit = false;
+      if (cut) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = row.qd_at(e[j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          bool keep = e[j] > -INFINITY;
-          if (least > -INFINITY) keep = keep && in_prefix(e[j], (uint32_t)(row.id0 + i + j));
-          if (!keep) q[j] = 0.0;
-          if (bounded) {
-            all_d += q[j];
-            const float t = row.t_of(e[j]);
-            hit |= keep && between(t);
-            keep = keep && t < t0;
-            above_d += keep ? q[j] : 0.0;
-          }
-          if (min_w > 0.0) keep = keep && row.w_of(e[j]) >= min_w;
-          else if (keep && e[j] <= row.low) keep = row.positive(e[j]);
-          sum += keep ? q[j] : 0.0;
-          n_thread += keep;
+        for (int j = 0; j < 4; ++j) if (!in_prefix(e[j], (uint32_t)(row.id0 + i + j))) e[j] = -INFINITY;
+        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > -INFINITY)) {
+          if (lane == 0) chunk[ch] = 0;
+          continue;
         }
-        if (__any_sync(0xffffffffu, hit)) {
-          bool hold[4];
-          unsigned votes[4];
-          int n_held = 0, at = 0;
+      }
+      double q[4], sum = 0.0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hold[j] = hit && e[j] > -INFINITY && between(row.t_of(e[j])) && in_prefix(e[j], (uint32_t)(row.id0 + i + j));
-            votes[j] = __ballot_sync(0xffffffffu, hold[j]);
-            n_held += __popc(votes[j]);
-          }
-          if (lane == 0) at = atomicAdd(&s->held_n, n_held);               // one a warp: single ones crowd the one address (13k cycles)
-          at = __shfl_sync(0xffffffffu, at, 0);
+      for (int j = 0; j < 4; ++j) q[j] = row.qd_at(e[j]);
+      unsigned hold = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (hold[j]) {
-              const int to = at + __popc(votes[j] & ((1u << lane) - 1));
-              row.add(fine_bin(row.t_of(e[j])), (u64)q[j]);
-              if (to < HELD) s->held[to] = make_uint2(key_of(e[j]), (uint32_t)(row.id0 + i + j));
-            }
-            at += __popc(votes[j]);
-          }
+      for (int j = 0; j < 4; ++j) {
+        bool in = e[j] >= v_above;
+        if (bounded) {
+          all_d += q[j];
+          hold |= (unsigned)(e[j] >= v_from && !in) << j;
         }
+        if (min_w > 0.0) {
+          above_d += in ? q[j] : 0.0;
+          in = in && row.w_of(e[j]) >= min_w;
+        } else if (look) in = in && row.positive(e[j]);
+        sum += in ? q[j] : 0.0;
+        n_thread += in;
+      }
+      if (bounded && __any_sync(0xffffffffu, hold)) {
+        const int n_lane = __popc(hold);
+        int at = n_lane;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += t; }
+        int base = 0;
+        if (lane == 31) base = atomicAdd(&s->held_n, at);                  // one a warp: single ones crowd the one address
+        at += __shfl_sync(0xffffffffu, base, 31) - n_lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (hold >> j & 1) { if (at < HELD) s->held[at] = make_uint2(key_of(e[j]), (uint32_t)(row.id0 + i + j)); ++at; }
       }
       const u64 in_chunk = warp_add((u64)sum);
       if (lane == 0) chunk[ch] = in_chunk;
+      if (min_w == 0.0 && lane == 0) above += in_chunk;
     }
-    above = (u64)above_d; all_q = (u64)all_d; n_kept = n_thread;
+    if (min_w > 0.0) above = (u64)above_d;
+    all_q = (u64)all_d; n_kept = n_thread;
   };
   weigh(by_p);
   if (by_p) {
     above = block_add(above, s->red); all_q = block_add(all_q, s->red);
-    const bool held_all = s->held_n <= HELD;
+    const bool held_all = s->held_n <= HELD;                 // else the ids between the bounds are looked up again
+    if (held_all) { for (int i = tid; i < s->held_n; i += THREADS) { const float v = value_of(s->held[i].x); row.add(fine_bin(v), row.q_at(v)); } }
+    else row.each(fmaxf(v_from, least), [&](float v, int i) { if (v < v_above && in_prefix(v, (uint32_t)(row.id0 + i))) row.add(fine_bin(v), row.q_at(v)); });
     const Mail *all = row.g.exchange(above | (held_all ? 0 : 1ull << 63), all_q);      // its sync also completes the histograms
     above = all_q = 0;
-    bool held = true;                                        // every CTA holds all its ids between the bounds
+    bool held = true;
 #pragma unroll
     for (int r = 0; r < C; ++r) { above += all[r].a & ~(1ull << 63); all_q += all[r].b; held = held && !(all[r].a >> 63); }
     const double target = fmax(frac * (double)all_q, 0.5);
@@ -639,7 +662,7 @@ sample_given_kernel(GivenArgs a) {
     row.counts(s->cnt, c); row.weights(m);
     const Found f = row.search(c, m, true, target, 0, above);
     const float k_least = least;
-    const Border bd = row.settle(fmaxf(row.below(b1), k_least), held, [&](float v, uint32_t) { const float t = row.t_of(v); return v >= k_least && between(t) && fine_bin(t) == f.bin; }, f, true, target);
+    const Border bd = row.settle(fmaxf(v_from, k_least), held, [&](float v, uint32_t) { return v >= k_least && v >= v_from && v < v_above && fine_bin(v) == f.bin; }, f, true, target);
     least = value_of(bd.key); last_id = bd.last_id;
     if (held) {                                              // the held ids that stay join their chunks
       for (int i = tid; i < s->held_n; i += THREADS) {
@@ -651,6 +674,7 @@ sample_given_kernel(GivenArgs a) {
         }
       }
     } else {
+      v_above = -FLT_MAX;
       weigh(false);
     }
   }
@@ -671,7 +695,7 @@ sample_given_kernel(GivenArgs a) {
   __syncthreads();
   if (before <= target && target < before + mine) {
     int ch = tid * per;
-    while (before + chunk[ch] <= target) before += chunk[ch++];
+    while (ch + 1 < n_chunks && before + chunk[ch] <= target) before += chunk[ch++];
     s->pick_chunk = ch; s->pick_before = before;
   }
   __syncthreads();
