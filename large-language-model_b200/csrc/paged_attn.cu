@@ -178,8 +178,8 @@ paged_join_kernel(PagedAttnArgs a) {
   const int group = tid / width, k0 = (int)((long long)parts * group / groups), k1 = (int)((long long)parts * (group + 1) / groups);
   for (int i0 = blockIdx.y * width; i0 < items; i0 += gridDim.y * width) {
     const int i = i0 + tid % width;
-    const int r = a.columns ? i % a.slot_rows : i / vecs, v = a.columns ? i / a.slot_rows : i - r * vecs, d = v * 4;
-    const size_t at = a.columns ? ((size_t)v * a.slot_rows + r) * 4 : (size_t)r * hd + d;
+    const int r = i / vecs, d = (i - r * vecs) * 4;
+    const size_t at = (size_t)r * hd + d;
     int row = 0, head = 0, pos = 0;
     const bool has = i < items && paged_row(a, pl, r, row, head, pos);
     const bool vec = hd % 4 == 0;
@@ -237,9 +237,14 @@ paged_join_kernel(PagedAttnArgs a) {
     }
     if (has && group == 0) {
       const float inv = l > 0.f ? 1.0f / l : 0.f;
+      T *dst = (T *)a.o + (size_t)row * a.ld_o + (size_t)head * hd + d;
+      if (a.vec_out && sizeof(T) == 2) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0] * inv, e[1] * inv), hi = __floats2bfloat162_rn(e[2] * inv, e[3] * inv);
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+      } else {
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (d + x < hd) ((T *)a.o)[(size_t)row * a.ld_o + (size_t)head * hd + d + x] = from_f<T>(e[x] * inv);
+        for (int x = 0; x < 4; ++x) if (d + x < hd) dst[x] = from_f<T>(e[x] * inv);
+      }
       if (a.lse && d == 0) a.lse[(size_t)row * a.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
     }
   }
@@ -322,8 +327,9 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
     }
   }
   if (paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o)) return paged_attn_tc_launch(ctx, a, G, few + 1);
-  a.plan = paged::Plan{G, 0, ROWS, TILE, 1, few + 1, 0x7fffffff};
-  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS; a.columns = 0;
+  a.vec_out = 0;
+  a.plan = paged::Plan{G, 0, ROWS, TILE, 1, few + 1, 0x7fffffff, 0};
+  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
   const bool big = cache->head_dim > 128;
   if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
   else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);
@@ -354,14 +360,14 @@ extern "C" int b200_internal_paged_probe(const b200_paged_cache *cache, const b2
   return B200_OK;
 }
 // Steps through the runs of all CTAs; writes (CTA, sequence, KV head, block, tile, whole block, parts to join at the CTA's border) per tile, returns how many.
-extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile, int extra,
+extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile, int extra, int halves,
                                                int lo, int hi, int n_cta, int min_units, int *out, long long room) {
   int status = 0;
   b200_ctx ctx;
   PagedArgs a;
   if (paged_args(&ctx, cache, batch, &a)) return -1;
   a.status = &status;
-  const paged::Plan p{G, tokens, rows, tile, extra, lo, hi};
+  const paged::Plan p{G, tokens, rows, tile, extra, lo, hi, halves};
   long long total = 0, n_out = 0;
   for (int s = 0; s < a.n_seq; ++s) total += paged::seq_units(a, p, s);
   if (total == 0) return 0;

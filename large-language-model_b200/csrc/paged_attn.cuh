@@ -9,7 +9,8 @@ struct PagedAttnArgs {
   void *o;
   float *lse, *ws;                       // ws: the join's heads, then the partial results
   long long ld_q, ld_o;
-  int nH, n_cta, min_units, slot_rows, columns;   // slot_rows: rows of one partial result
+  int nH, n_cta, min_units, slot_rows;   // slot_rows: rows of one partial result
+  int vec_out;                           // rows of o are 16-byte aligned
   float scale;
 };
 
@@ -17,7 +18,6 @@ constexpr int PAGED_FEW_ROWS = 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 // Partial result of a block: [slot_rows][hd] output in units of 2^maximum, then [slot_rows] maxima (log2 units), [slot_rows] sums.
-// With `columns` the output is laid out [hd / 4][slot_rows][4] instead (threads that each own a row write whole segments).
 // A part whose maximum is -inf saw no key; its output is not read.  CTA c owns two: slot 2c for a block that began before its run, 2c + 1 for one that begins in it and ends behind it.
 __host__ __device__ __forceinline__ size_t paged_slot_floats(int slot_rows, int hd) { return (size_t)slot_rows * (hd + 2); }
 // What the join needs of the border before run c: written by CTA c (every CTA of the grid writes its own).

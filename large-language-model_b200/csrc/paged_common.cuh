@@ -69,12 +69,13 @@ __host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int p
 // ---- division of the work ---------------------------------------------------------------------------------------------
 // A sequence's rows (token, query head of the group) are cut into blocks; a block walks the key tiles its last row can see.
 // All (sequence, KV head, block, tile) in this order form one line; a block takes `extra` units (its start and end, in tiles' time)
-// and one per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
+// and `cost` per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
 // whatever the lengths are (without the extra, CTAs whose run held dozens of short sequences took 1.8 times the others' time).
 // A block that crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
 struct Plan {
   int G, tokens_per_block, rows_per_block;   // rows_per_block > 0: blocks of consecutive rows; else blocks of whole tokens
   int tile, extra, min_rows, max_rows;       // keys per tile; only sequences with min_rows <= rows <= max_rows take part
+  int halves;                                // 1: a tile costs two units in blocks with rows in both halves of their tokens, else one
   __host__ __device__ __forceinline__ bool takes(int ql) const { const long long r = (long long)ql * G; return ql > 0 && r >= min_rows && r <= max_rows; }
   __host__ __device__ __forceinline__ int blocks(int ql) const {
     return rows_per_block ? (int)(((long long)ql * G + rows_per_block - 1) / rows_per_block) : (ql + tokens_per_block - 1) / tokens_per_block;
@@ -86,13 +87,18 @@ struct Plan {
     return greater(1, (seen + tile - 1) / tile);   // a block that sees nothing still writes its empty rows
   }
 };
+// log2 of a tile's cost
+__host__ __device__ __forceinline__ int tile_shift(const Plan &p, const Seq &q, int block) {
+  return p.halves && (long long)block * p.tokens_per_block + p.tokens_per_block / 2 < q.ql ? 1 : 0;
+}
+__host__ __device__ __forceinline__ long long block_units(const Plan &p, const Seq &q, int block) { return ((long long)p.tiles(q, block) << tile_shift(p, q, block)) + p.extra; }
 struct Place { int seq, kvh, block, kt; Seq q; long long first; };   // tile kt of a block, which begins at unit `first`
 
 __host__ __device__ __forceinline__ long long seq_units(const PagedArgs &a, const Plan &p, int s) {
   const Seq q = load_seq(a, s);
   if (!p.takes(q.ql)) return 0;
   long long u = 0;
-  for (int b = p.blocks(q.ql) - 1; b >= 0; --b) u += p.tiles(q, b) + p.extra;
+  for (int b = p.blocks(q.ql) - 1; b >= 0; --b) u += block_units(p, q, b);
   return u * a.n_kv;
 }
 
@@ -102,9 +108,10 @@ __host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Pla
   Place pl;
   pl.seq = s; pl.q = load_seq(a, s); pl.kvh = (int)((u - at) / per_head);
   pl.first = at + pl.kvh * per_head;
-  int b = 0, t = p.tiles(pl.q, 0) + p.extra;
-  while (u - pl.first >= t) { pl.first += t; t = p.tiles(pl.q, ++b) + p.extra; }
-  pl.block = b; pl.kt = greater(0, (int)(u - pl.first) - p.extra);
+  int b = 0;
+  long long t = block_units(p, pl.q, 0);
+  while (u - pl.first >= t) { pl.first += t; t = block_units(p, pl.q, ++b); }
+  pl.block = b; pl.kt = greater(0, (int)(u - pl.first) - p.extra) >> tile_shift(p, pl.q, b);
   return pl;
 }
 
@@ -124,7 +131,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long *red, lon
   return before + inc - v;
 }
 
-// CTAs that take part: at most n_max, and few enough that each gets min_units.
+// CTAs that take part: at most n_max, and few enough that each gets min_units (at least the cost of a tile, so that a run between two
+// others inside a block is never empty).
 __host__ __device__ __forceinline__ int line_ctas(long long total, int n_max, int min_units) {
   const long long n = (total + min_units - 1) / min_units;
   return n < 1 ? 1 : n < n_max ? (int)n : n_max;
@@ -171,13 +179,13 @@ struct Walk {
   __host__ __device__ __forceinline__ void start(const Plan &p, const Place &at, long long end) { pl = at; set(p, end); }
   __host__ __device__ __forceinline__ void set(const Plan &p, long long end) {
     tiles = p.tiles(pl.q, pl.block);
-    const long long room = end - pl.first - p.extra;
+    const long long room = (end - pl.first - p.extra) >> tile_shift(p, pl.q, pl.block);      // rounds like the next CTA's start
     k1 = room < tiles ? (int)room : tiles;
     more = k1 > pl.kt;                                     // a run that ends in a block's extra leaves it to the next CTA
   }
   __host__ __device__ __forceinline__ bool whole() const { return pl.kt == 0 && k1 == tiles; }
   __host__ __device__ __forceinline__ void next(const PagedArgs &a, const Plan &p, long long end) {
-    pl.first += tiles + p.extra;
+    pl.first += block_units(p, pl.q, pl.block);
     pl.kt = 0;
     if (pl.first >= end) { more = false; return; }
     if (++pl.block >= p.blocks(pl.q.ql)) {
@@ -196,8 +204,8 @@ struct Walk {
 };
 // How many CTAs, from c - 1 on, have parts of the block that run c begins in; 0 unless c is the first border inside that block.
 __host__ __device__ __forceinline__ int parts_at(const Plan &p, const Run &r, const Place &pl, int c) {
-  if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) > pl.first + p.extra) return 0;
-  const long long last = pl.first + p.extra + p.tiles(pl.q, pl.block), c1 = (last * r.n - 1) / r.total;      // line_at(c1) < last
+  if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) >= pl.first + p.extra + (1 << tile_shift(p, pl.q, pl.block))) return 0;
+  const long long last = pl.first + block_units(p, pl.q, pl.block), c1 = (last * r.n - 1) / r.total;      // line_at(c1) < last
   return (int)(c1 < r.n - 1 ? c1 : r.n - 1) - c + 2;
 }
 
