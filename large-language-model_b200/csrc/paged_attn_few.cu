@@ -270,7 +270,7 @@ bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t l
 
 int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G) {
   const bool two = (long long)a.b.max_q * G > 16;
-  a.plan = paged::Plan{G, 0, two ? 32 : 16, TILE, 2, 0, two ? PAGED_FEW_ROWS : 16, 0};
+  a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 2, 0, two ? PAGED_FEW_ROWS : 16, 0};
   a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);
   return two ? launch_t<64, 2>(ctx, a) : launch_t<64, 1>(ctx, a);

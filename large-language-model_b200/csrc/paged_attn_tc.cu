@@ -475,7 +475,7 @@ bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const vo
 }
 
 int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs a, int G, int min_rows) {
-  a.plan = paged::Plan{G, 2 * (128 / G), 0, TK, 2, min_rows, 0x7fffffff, 1};
+  a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 2, min_rows, 0x7fffffff, 1};
   a.n_cta = ctx->sm_count; a.min_units = 4; a.slot_rows = 256; a.vec_out = 1;
   return a.b.hd == 128 ? launch_t<128>(ctx, a) : launch_t<64>(ctx, a);
 }

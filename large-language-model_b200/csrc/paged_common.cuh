@@ -74,17 +74,25 @@ __host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int p
 // A block that crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
 struct Plan {
   int G, tokens_per_block, rows_per_block;   // rows_per_block > 0: blocks of consecutive rows; else blocks of whole tokens
-  int tile, extra, min_rows, max_rows;       // keys per tile; only sequences with min_rows <= rows <= max_rows take part
+  int tile_log2, extra, min_rows, max_rows;  // keys per tile; only sequences with min_rows <= rows <= max_rows take part
   int halves;                                // 1: a tile costs two units in blocks with rows in both halves of their tokens, else one
   __host__ __device__ __forceinline__ bool takes(int ql) const { const long long r = (long long)ql * G; return ql > 0 && r >= min_rows && r <= max_rows; }
   __host__ __device__ __forceinline__ int blocks(int ql) const {
-    return rows_per_block ? (int)(((long long)ql * G + rows_per_block - 1) / rows_per_block) : (ql + tokens_per_block - 1) / tokens_per_block;
+    if (max_rows <= rows_per_block) return 1;
+    if (!rows_per_block) return (int)((unsigned)(ql + tokens_per_block - 1) / (unsigned)tokens_per_block);
+    const unsigned long long r = (unsigned long long)ql * G + rows_per_block - 1;
+    return r >> 32 ? (int)(r / rows_per_block) : (int)((unsigned)r / (unsigned)rows_per_block);      // (a 64-bit division costs a microsecond in a loop)
   }
   __host__ __device__ __forceinline__ int tiles(const Seq &q, int block) const {
-    const long long end = rows_per_block ? ((long long)(block + 1) * rows_per_block - 1) / G + 1 : (long long)(block + 1) * tokens_per_block;
-    const int last = (int)(end < q.ql ? end : q.ql) - 1;
-    const int seen = lesser(greater(q.base + last + 1, 0), q.len);
-    return greater(1, (seen + tile - 1) / tile);   // a block that sees nothing still writes its empty rows
+    int last = q.ql;                                                     // rows up to the block's end
+    if (!rows_per_block) { const long long end = (long long)(block + 1) * tokens_per_block; last = end < q.ql ? (int)end : q.ql; }
+    else if (max_rows > rows_per_block) {
+      const unsigned long long r = (unsigned long long)(block + 1) * rows_per_block - 1;
+      const unsigned long long end = (r >> 32 ? r / G : (unsigned)r / (unsigned)G) + 1;
+      last = end < (unsigned long long)q.ql ? (int)end : q.ql;
+    }
+    const int seen = lesser(greater(q.base + last, 0), q.len);
+    return greater(1, (int)(((long long)seen + (1 << tile_log2) - 1) >> tile_log2));   // a block that sees nothing still writes its empty rows
   }
 };
 // log2 of a tile's cost

@@ -161,7 +161,7 @@ def cover(lib, q_lens, kv_lens, n_kv, G, few, n_cta, min_units):
     c = cache(n_pages=1, page_size=1, n_kv=n_kv, head_dim=1, head_stride=1, token_stride=1, page_stride=1)
     b = bridge._PagedBatch(q_start.ctypes.data, kv.ctypes.data, table.ctypes.data, kv.size, table.shape[1], int(q_start[-1]), 0)
     out = np.empty((200000, 7), np.int32)
-    n = fn(C.byref(c), C.byref(b), G, few["tokens"], few["rows"], few["tile"], few["extra"], few["halves"], few["lo"], few["hi"], n_cta, min_units, out.ctypes.data, len(out))
+    n = fn(C.byref(c), C.byref(b), G, few["tokens"], few["rows"], int(np.log2(few["tile"])), few["extra"], few["halves"], few["lo"], few["hi"], n_cta, min_units, out.ctypes.data, len(out))
     assert 0 <= n <= len(out)
     return out[:n]
 
