@@ -23,7 +23,7 @@ template <class T, int HJ>
 __global__ void __launch_bounds__(THREADS)
 paged_attn_simt_kernel(PagedAttnArgs a) {
   pdl_wait();
-  pdl_launch_dependents();                     // behind the wait: the join may read the batch as soon as it starts
+  pdl_launch_dependents();
   extern __shared__ __align__(16) float smem[];
   __shared__ long long red[33];
   __shared__ paged::Place place;
@@ -162,12 +162,14 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
 template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS)
-paged_join_kernel(PagedAttnArgs a) {
+paged_join_kernel(PagedAttnArgs a, PagedAttnArgs a2) {
   pdl_wait();
   pdl_launch_dependents();
+  int c = blockIdx.x + 1;
+  if (c >= a.n_cta) { c -= a.n_cta - 1; a = a2; }      // the second kernel's borders follow the first's
   __shared__ float sh_m[JOIN_WARPS][32], sh_l[JOIN_WARPS][32];
   __shared__ float4 sh_e[JOIN_WARPS][32];
-  const int c = blockIdx.x + 1, hd = a.b.hd, tid = threadIdx.x;
+  const int hd = a.b.hd, tid = threadIdx.x;
   const JoinHead *head_ = paged_head(a, c);
   const int parts = head_->parts;
   if (parts == 0) return;
@@ -266,21 +268,21 @@ constexpr int MIN_UNITS = 4;
 
 }  // namespace
 
-int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt) {
-  if (a.n_cta < 2) return B200_OK;
-  const int work = a.slot_rows * ((a.b.hd + 3) / 4);
-  const dim3 grid((unsigned)(a.n_cta - 1), (unsigned)std::min(16, (work + JOIN_THREADS - 1) / JOIN_THREADS));
+int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, const PagedAttnArgs *b, b200_dtype dt) {
+  const int borders = a.n_cta - 1 + (b ? b->n_cta - 1 : 0), rows = std::max(a.slot_rows, b ? b->slot_rows : 0);
+  if (borders < 1) return B200_OK;
+  const dim3 grid((unsigned)borders, (unsigned)std::min(16, (rows * ((a.b.hd + 3) / 4) + JOIN_THREADS - 1) / JOIN_THREADS));
   const bool pdl = ctx->pdl;
-  ctx->pdl = true;                             // the join's set-up overlaps the end of the kernel before it
-  const cudaError_t e = dt == B200_BF16 ? launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a)
-                                        : launch_k(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a);
+  ctx->pdl = true;                             // its launch overlaps the end of the kernel before, which itself ends after the one it ran beside
+  const cudaError_t e = dt == B200_BF16 ? launch_k(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a)
+                                        : launch_k(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a);
   ctx->pdl = pdl;
   B200_CUDA(ctx, e);
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
 
-// Each kernel leaves two partial results per CTA; the kernels of one call follow each other, so they share the room.
+// Each kernel leaves two partial results per CTA; two kernels of one call may run side by side, so each has its own room.
 static size_t partial_bytes(const b200_ctx *ctx, int ctas_per_sm, int slot_rows, size_t hd) {
   return (size_t)ctas_per_sm * ctx->sm_count * (JOIN_HEAD_FLOATS + 2 * paged_slot_floats(slot_rows, (int)hd)) * sizeof(float);
 }
@@ -292,7 +294,8 @@ extern "C" int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *
   if (rc) return rc;
   B200_REQUIRE(ctx, bytes, "paged_attn_workspace: null pointer");
   B200_REQUIRE(ctx, n_heads > 0 && n_heads <= 65536 && n_heads % cache->n_kv == 0, "paged_attn: n_heads must be a multiple of the cache's n_kv");
-  *bytes = std::max(partial_bytes(ctx, 2, ROWS, cache->head_dim), cache->dtype == B200_BF16 && cache->head_dim <= 128 ? partial_bytes(ctx, 1, 256, cache->head_dim) : 0);
+  const size_t hd = cache->head_dim;
+  *bytes = partial_bytes(ctx, 2, ROWS, hd) + (cache->dtype == B200_BF16 && hd <= 128 ? partial_bytes(ctx, 1, 256, hd) : 0);
   return B200_OK;
 }
 
@@ -316,25 +319,28 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
   a.ld_q = (long long)ld_q; a.ld_o = (long long)ld_o; a.nH = (int)n_heads;
   a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)cache->head_dim);
   const int G = (int)(n_heads / cache->n_kv);
-  int few = 0;                                  // sequences of up to this many rows are taken by the few-row kernel
-  if (paged_attn_few_supported(cache, q, ld_q, o, ld_o)) {
-    // A lone sequence or two with many rows are not worth a launch that will find nothing (each kernel is right for any row count).
-    const long long most = (long long)a.b.max_q * G;
-    if (most <= PAGED_FEW_ROWS || a.b.n_seq > 2) {
-      rc = paged_attn_few_launch(ctx, a, G);
-      if (rc || most <= PAGED_FEW_ROWS) return rc;
-      few = PAGED_FEW_ROWS;
+  const bool big = cache->head_dim > 128, fast = paged_attn_few_supported(cache, q, ld_q, o, ld_o), tc = fast && paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o);
+  // Sequences of up to PAGED_FEW_ROWS rows are the few-row kernel's, the others the chunk kernel's (tcgen05, else CUDA cores).  A lone sequence or
+  // two with many rows are not worth a launch that will find nothing (each kernel is right for any row count).
+  const long long most = (long long)a.b.max_q * G;
+  const bool few = fast && (most <= PAGED_FEW_ROWS || a.b.n_seq > 2), many = !fast || most > PAGED_FEW_ROWS;
+  PagedAttnArgs f = a;
+  if (many) {
+    if (tc) rc = paged_attn_tc_launch(ctx, a, G, few ? PAGED_FEW_ROWS + 1 : 0);
+    else {
+      a.vec_out = 0; a.beside = 0;
+      a.plan = paged::Plan{G, 0, ROWS, 5, 1, few ? PAGED_FEW_ROWS + 1 : 0, 0x7fffffff, 0};
+      a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
+      if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
+      else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);
     }
+    if (rc) return rc;
+    if (!few) return paged_join_launch(ctx, a, nullptr, cache->dtype);
+    f.ws = a.ws + (size_t)a.n_cta * (JOIN_HEAD_FLOATS + 2 * paged_slot_floats(a.slot_rows, a.b.hd));
   }
-  if (paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o)) return paged_attn_tc_launch(ctx, a, G, few + 1);
-  a.vec_out = 0;
-  a.plan = paged::Plan{G, 0, ROWS, 5, 1, few + 1, 0x7fffffff, 0};
-  a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
-  const bool big = cache->head_dim > 128;
-  if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
-  else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);
+  rc = paged_attn_few_launch(ctx, f, G, many);
   if (rc) return rc;
-  return paged_join_launch(ctx, a, cache->dtype);
+  return many ? paged_join_launch(ctx, a, &f, cache->dtype) : paged_join_launch(ctx, f, nullptr, cache->dtype);
 }
 
 // Test hooks, on the host, over host arrays: what the kernels' own index code reaches.

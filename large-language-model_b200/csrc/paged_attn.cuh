@@ -11,6 +11,7 @@ struct PagedAttnArgs {
   long long ld_q, ld_o;
   int nH, n_cta, min_units, slot_rows;   // slot_rows: rows of one partial result
   int vec_out;                           // rows of o are 16-byte aligned
+  int beside;                            // do not wait for the kernel before
   float scale;
 };
 
@@ -50,8 +51,12 @@ __device__ __forceinline__ bool paged_row(const PagedAttnArgs &a, const paged::P
   return tok < pl.q.ql;
 }
 
-int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, b200_dtype dt);
+// Joins what one or two kernels left (b may be null).
+int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, const PagedAttnArgs *b, b200_dtype dt);
 bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t ld_q, const void *o, size_t ld_o);
-int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G);   // the kernel and its join
+// The launchers complete `a` (the join needs it); its workspace begins at a.ws.
+// beside: the kernel before it on the stream works on other sequences of the same call and has waited for what came before the call, so this one
+// starts without waiting and fills the SMs that the other leaves; it waits for the other before it ends, so that what follows it follows both.
+int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, bool beside);
 bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const void *q, size_t ld_q, const void *o, size_t ld_o);
-int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs a, int G, int min_rows);   // the kernel and its join
+int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, int min_rows);

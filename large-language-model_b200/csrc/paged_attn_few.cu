@@ -45,8 +45,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <int HD, int MT>
 __global__ void __launch_bounds__(THREADS, 2)
 paged_attn_few_kernel(PagedAttnArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();                     // behind the wait: the join may read the batch as soon as it starts
+  if (!a.beside) pdl_wait();
+  pdl_launch_dependents();
   constexpr int CH = HD / 8, KS = HD / 16, NT = HD / 8;        // 16-byte chunks of a row, k steps of the scores, n tiles of the output
   constexpr int ROW = HD * 2, HALF = SLICE * ROW, STAGE = 2 * HALF, OST = HD + 4;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -57,7 +57,7 @@ paged_attn_few_kernel(PagedAttnArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, c = blockIdx.x;
   const paged::Run run = paged::line_run<THREADS>(a.b, a.plan, c, a.n_cta, a.min_units, red, &place);
   if (tid == 0) paged_write_head(a, run, place, c);
-  if (run.u == run.end) return;
+  if (run.u == run.end) { if (a.beside) pdl_wait(); return; }
   uint8_t *ring = smem + warp * STAGES * STAGE;
   const float sl2 = a.scale * PAGED_LOG2E;
 
@@ -247,6 +247,7 @@ paged_attn_few_kernel(PagedAttnArgs a) {
       __syncthreads();
     }
   }
+  if (a.beside) pdl_wait();
 }
 
 template <int HD, int MT>
@@ -255,9 +256,13 @@ int launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
   if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_few_kernel<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr.fetch_or(bit); }
-  B200_CUDA(ctx, launch_k(ctx, paged_attn_few_kernel<HD, MT>, dim3((unsigned)a.n_cta), dim3(THREADS), (size_t)smem, 0, a));
+  const bool pdl = ctx->pdl;
+  ctx->pdl = pdl || a.beside;
+  const cudaError_t e = launch_k(ctx, paged_attn_few_kernel<HD, MT>, dim3((unsigned)a.n_cta), dim3(THREADS), (size_t)smem, 0, a);
+  ctx->pdl = pdl;
+  B200_CUDA(ctx, e);
   B200_LAUNCHED(ctx);
-  return paged_join_launch(ctx, a, B200_BF16);
+  return B200_OK;
 }
 
 }  // namespace
@@ -268,10 +273,10 @@ bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t l
   return ((uintptr_t)q | (uintptr_t)o | (uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0 && (ld_q | ld_o | c->page_stride | c->token_stride | c->head_stride) % 8 == 0;
 }
 
-int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs a, int G) {
+int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, bool beside) {
   const bool two = (long long)a.b.max_q * G > 16;
   a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 2, 0, two ? PAGED_FEW_ROWS : 16, 0};
-  a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1;
+  a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1; a.beside = beside ? 1 : 0;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);
   return two ? launch_t<64, 2>(ctx, a) : launch_t<64, 1>(ctx, a);
 }

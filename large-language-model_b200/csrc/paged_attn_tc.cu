@@ -86,7 +86,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int *abort_flag = &sh->abort_flag;
   pdl_wait();
-  pdl_launch_dependents();                       // behind the wait: the join may read the batch as soon as it starts
+  pdl_launch_dependents();                       // behind the wait: a few-row kernel that follows does not wait for this one
   const paged::Run run = paged::line_run<TC_THREADS>(a.b, a.plan, blockIdx.x, a.n_cta, a.min_units, sh->red, &sh->place);
   if (threadIdx.x == 0) paged_write_head(a, run, sh->place, blockIdx.x);
   if (run.u == run.end) return;
@@ -463,7 +463,7 @@ int launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
   if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr.fetch_or(bit); }
   B200_CUDA(ctx, launch_k(ctx, paged_attn_tc_kernel<HD>, dim3((unsigned)a.n_cta), dim3(TC_THREADS), (size_t)smem, 0, mq, mk, mv, a, box));
   B200_LAUNCHED(ctx);
-  return paged_join_launch(ctx, a, B200_BF16);
+  return B200_OK;
 }
 
 }  // namespace
@@ -474,8 +474,8 @@ bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const vo
   return paged_attn_few_supported(c, q, ld_q, o, ld_o) && c->page_size % 8 == 0 && n_heads / c->n_kv <= 128;
 }
 
-int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs a, int G, int min_rows) {
-  a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 2, min_rows, 0x7fffffff, 1};
-  a.n_cta = ctx->sm_count; a.min_units = 4; a.slot_rows = 256; a.vec_out = 1;
+int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, int min_rows) {
+  a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 6, min_rows, 0x7fffffff, 1};
+  a.n_cta = ctx->sm_count; a.min_units = 4; a.slot_rows = 256; a.vec_out = 1; a.beside = 0;
   return a.b.hd == 128 ? launch_t<128>(ctx, a) : launch_t<64>(ctx, a);
 }

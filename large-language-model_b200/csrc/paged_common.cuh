@@ -95,6 +95,8 @@ struct Plan {
     return greater(1, (int)(((long long)seen + (1 << tile_log2) - 1) >> tile_log2));   // a block that sees nothing still writes its empty rows
   }
 };
+// Divisions of positions on the line are 32-bit ones wherever it is that short.
+__host__ __device__ __forceinline__ long long quotient(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
 // log2 of a tile's cost
 __host__ __device__ __forceinline__ int tile_shift(const Plan &p, const Seq &q, int block) {
   return p.halves && (long long)block * p.tokens_per_block + p.tokens_per_block / 2 < q.ql ? 1 : 0;
@@ -112,9 +114,9 @@ __host__ __device__ __forceinline__ long long seq_units(const PagedArgs &a, cons
 
 // Unit u of the line, which is in sequence s, whose units begin at `at` and number `units`.
 __host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Plan &p, int s, long long units, long long at, long long u) {
-  const long long per_head = units / a.n_kv;
+  const long long per_head = quotient(units, a.n_kv);
   Place pl;
-  pl.seq = s; pl.q = load_seq(a, s); pl.kvh = (int)((u - at) / per_head);
+  pl.seq = s; pl.q = load_seq(a, s); pl.kvh = per_head >> 31 ? (int)((u - at) / per_head) : (int)quotient(u - at, (int)per_head);
   pl.first = at + pl.kvh * per_head;
   int b = 0;
   long long t = block_units(p, pl.q, 0);
@@ -142,11 +144,21 @@ __device__ __forceinline__ long long block_scan(long long v, long long *red, lon
 // CTAs that take part: at most n_max, and few enough that each gets min_units (at least the cost of a tile, so that a run between two
 // others inside a block is never empty).
 __host__ __device__ __forceinline__ int line_ctas(long long total, int n_max, int min_units) {
-  const long long n = (total + min_units - 1) / min_units;
+  const long long n = quotient(total, min_units);        // (rounded down: no CTA gets less)
   return n < 1 ? 1 : n < n_max ? (int)n : n_max;
 }
-__host__ __device__ __forceinline__ long long line_at(long long total, int n, int c) { return total * c / n; }
-
+__host__ __device__ __forceinline__ long long line_at(long long total, int n, int c) {      // the first total % n CTAs have one unit more
+  const long long each = quotient(total, n);
+  const int more = (int)(total - each * n);
+  return each * c + lesser(c, more);
+}
+__host__ __device__ __forceinline__ int line_cta(long long total, int n, long long u) {      // the CTA of unit u
+  const long long each = quotient(total, n);
+  const int more = (int)(total - each * n);
+  const long long longer = (each + 1) * more;
+  return u < longer ? (int)((u >> 32) || each >> 31 ? u / (each + 1) : (unsigned)u / (unsigned)(each + 1))
+                    : more + (int)(((u - longer) >> 32) || each >> 31 ? (u - longer) / each : (unsigned)(u - longer) / (unsigned)each);
+}
 struct Run { long long u, end, total; int n; };          // units [u, end) of CTA c; n CTAs take part
 
 // The run of CTA c, and the place of unit u in *out (shared) unless the run is empty.  All threads must call; ends with a barrier.
@@ -213,8 +225,7 @@ struct Walk {
 // How many CTAs, from c - 1 on, have parts of the block that run c begins in; 0 unless c is the first border inside that block.
 __host__ __device__ __forceinline__ int parts_at(const Plan &p, const Run &r, const Place &pl, int c) {
   if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) >= pl.first + p.extra + (1 << tile_shift(p, pl.q, pl.block))) return 0;
-  const long long last = pl.first + block_units(p, pl.q, pl.block), c1 = (last * r.n - 1) / r.total;      // line_at(c1) < last
-  return (int)(c1 < r.n - 1 ? c1 : r.n - 1) - c + 2;
+  return line_cta(r.total, r.n, pl.first + block_units(p, pl.q, pl.block) - 1) - c + 2;
 }
 
 }  // namespace paged
