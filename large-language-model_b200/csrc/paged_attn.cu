@@ -18,8 +18,48 @@ namespace {
 
 constexpr int THREADS = 128, ROWS = 32, TILE = 32, WROWS = ROWS / 4;
 
+// Four elements in 32 bits.
+template <class T> __device__ __forceinline__ float4 load4(const T *p);
+template <> __device__ __forceinline__ float4 load4<float>(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+template <> __device__ __forceinline__ float4 load4<bf16>(const bf16 *p) {
+  const uint2 v = *reinterpret_cast<const uint2 *>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+// Copies rows of hd elements at src + off[row] into shared rows `stride` floats apart, zeros where off < 0 and up to the padded size hd4; UNROLL
+// vectors of a thread in flight (VEC: rows are four-element aligned), two sources at once.
+template <class T, bool VEC, int UNROLL, class A, class B>
+__device__ __forceinline__ void copy_rows(const T *src, const T *src2, const long long *off, int rows, int hd, A to, B to2) {
+  const int hd4 = (hd + 3) / 4, all = rows * hd4;
+  for (int i0 = threadIdx.x; i0 < all; i0 += UNROLL * THREADS) {
+    float4 x[UNROLL], y[UNROLL];
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = i0 + j * THREADS;
+      x[j] = y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < all) {
+        const int r = i / hd4, d = (i - r * hd4) * 4;
+        const long long o = off[r];
+        if (o >= 0) {
+          if constexpr (VEC) { x[j] = load4(src + o + d); if (src2) y[j] = load4(src2 + o + d); }
+          else {
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { e[k] = d + k < hd ? to_f(src[o + d + k]) : 0.f; e[4 + k] = src2 && d + k < hd ? to_f(src2[o + d + k]) : 0.f; }
+            x[j] = make_float4(e[0], e[1], e[2], e[3]); y[j] = make_float4(e[4], e[5], e[6], e[7]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = i0 + j * THREADS;
+      if (i < all) { const int r = i / hd4, d = (i - r * hd4) * 4; to(r, d, x[j]); if (src2) to2(r, d, y[j]); }
+    }
+  }
+}
+
 // HJ: 128-dimension slices of the head.
-template <class T, int HJ>
+template <class T, int HJ, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 paged_attn_simt_kernel(PagedAttnArgs a) {
   pdl_wait();
@@ -27,7 +67,8 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   __shared__ long long red[33];
   __shared__ paged::Place place;
-  __shared__ int page_s[TILE];
+  __shared__ long long off_s[TILE];                    // element offset of a key's row, or of a query's; -1: zeros
+  static_assert(TILE >= ROWS, "one table for keys and queries");
   const int hd = a.b.hd, hd4 = (hd + 3) & ~3, kst = hd4 + 4, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float *sK = smem, *sV = sK + TILE * kst, *sQ = sV + TILE * hd4, *sP = sQ + ROWS * hd4 + warp * WROWS * TILE;
   const int c = blockIdx.x;
@@ -40,13 +81,12 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
     const paged::Place &pl = w.pl;
     // ---- queries of the block, rows that do not exist as zeros
     __syncthreads();
-    for (int i = tid; i < ROWS * hd4; i += THREADS) {
-      const int r = i / hd4, d = i - r * hd4;
+    if (tid < ROWS) {
       int row, head, pos;
-      float x = 0.f;
-      if (paged_row(a, pl, r, row, head, pos) && d < hd) x = to_f(((const T *)a.q)[(size_t)row * a.ld_q + (size_t)head * hd + d]);
-      sQ[i] = x;
+      off_s[tid] = paged_row(a, pl, tid, row, head, pos) ? (long long)row * a.ld_q + (long long)head * hd : -1;
     }
+    __syncthreads();
+    copy_rows<T, VEC, 4>((const T *)a.q, (const T *)nullptr, off_s, ROWS, hd, [&](int r, int d, float4 x) { *reinterpret_cast<float4 *>(sQ + r * hd4 + d) = x; }, [](int, int, float4) {});
     int limit[WROWS], out_row[WROWS], out_head[WROWS], live = 0;      // limit: keys the row sees
     float m[WROWS], l[WROWS];
     float4 acc[WROWS][HJ];
@@ -62,20 +102,13 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
     }
     for (int kt = pl.kt; kt < w.k1; ++kt) {
       __syncthreads();
-      if (tid < TILE) {
-        const int pos = kt * TILE + tid;
-        page_s[tid] = pos < pl.q.len ? paged::page_of(a.b, pl.seq, pos) : -1;
+      if (tid < TILE) {                                                // positions never written may hold anything: read as zero
+        const int pos = kt * TILE + tid, page = pos < pl.q.len ? paged::page_of(a.b, pl.seq, pos) : -1;
+        off_s[tid] = page < 0 ? -1 : (long long)page * a.b.page_stride + (long long)(pos % a.b.page_size) * a.b.token_stride + (long long)pl.kvh * a.b.head_stride;
       }
       __syncthreads();
-      for (int i = tid; i < TILE * hd4; i += THREADS) {
-        const int r = i / hd4, d = i - r * hd4, page = page_s[r];
-        float x = 0.f, y = 0.f;                                        // positions never written may hold anything: read as zero
-        if (page >= 0 && d < hd) {
-          const long long at = (long long)page * a.b.page_stride + (long long)((kt * TILE + r) % a.b.page_size) * a.b.token_stride + (long long)pl.kvh * a.b.head_stride + d;
-          x = to_f(((const T *)a.k)[at]); y = to_f(((const T *)a.v)[at]);
-        }
-        sK[r * kst + d] = x; sV[i] = y;
-      }
+      copy_rows<T, VEC, 4>((const T *)a.k, (const T *)a.v, off_s, TILE, hd, [&](int r, int d, float4 x) { *reinterpret_cast<float4 *>(sK + r * kst + d) = x; },
+                           [&](int r, int d, float4 x) { *reinterpret_cast<float4 *>(sV + r * hd4 + d) = x; });
       __syncthreads();
       if (live == 0) continue;
       float s[WROWS];
@@ -252,19 +285,25 @@ paged_join_kernel(PagedAttnArgs a, PagedAttnArgs a2) {
   }
 }
 
-template <class T, int HJ>
-int simt_launch(b200_ctx *ctx, const PagedAttnArgs &a) {
+template <class T, int HJ, bool VEC>
+int simt_launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
   const int hd4 = (a.b.hd + 3) & ~3;
   const size_t smem = sizeof(float) * (size_t)(TILE * (hd4 + 4) + TILE * hd4 + ROWS * hd4 + ROWS * TILE);
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
-  if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_simt_kernel<T, HJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024)); attr.fetch_or(bit); }
-  B200_CUDA(ctx, launch_k(ctx, paged_attn_simt_kernel<T, HJ>, dim3((unsigned)a.n_cta), dim3(THREADS), smem, 0, a));
+  if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_simt_kernel<T, HJ, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024)); attr.fetch_or(bit); }
+  B200_CUDA(ctx, launch_k(ctx, paged_attn_simt_kernel<T, HJ, VEC>, dim3((unsigned)a.n_cta), dim3(THREADS), smem, 0, a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
+template <class T>
+int simt_launch(b200_ctx *ctx, const PagedAttnArgs &a) {
+  const bool vec = ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q) % (4 * sizeof(T)) == 0 && (a.b.page_stride | a.b.token_stride | a.b.head_stride | a.ld_q | a.b.hd) % 4 == 0;
+  if (a.b.hd > 128) return vec ? simt_launch_t<T, 2, true>(ctx, a) : simt_launch_t<T, 2, false>(ctx, a);
+  return vec ? simt_launch_t<T, 1, true>(ctx, a) : simt_launch_t<T, 1, false>(ctx, a);
+}
 
-constexpr int MIN_UNITS = 4;
+constexpr int MIN_UNITS = 1;
 
 }  // namespace
 
@@ -319,7 +358,7 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
   a.ld_q = (long long)ld_q; a.ld_o = (long long)ld_o; a.nH = (int)n_heads;
   a.scale = scale > 0.f ? scale : 1.0f / sqrtf((float)cache->head_dim);
   const int G = (int)(n_heads / cache->n_kv);
-  const bool big = cache->head_dim > 128, fast = paged_attn_few_supported(cache, q, ld_q, o, ld_o), tc = fast && paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o);
+  const bool fast = paged_attn_few_supported(cache, q, ld_q, o, ld_o), tc = fast && paged_attn_tc_supported(cache, n_heads, q, ld_q, o, ld_o);
   // Sequences of up to PAGED_FEW_ROWS rows are the few-row kernel's, the others the chunk kernel's (tcgen05, else CUDA cores).  A lone sequence or
   // two with many rows are not worth a launch that will find nothing (each kernel is right for any row count).
   const long long most = (long long)a.b.max_q * G;
@@ -331,8 +370,7 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
       a.vec_out = 0; a.beside = 0;
       a.plan = paged::Plan{G, 0, ROWS, 5, 1, few ? PAGED_FEW_ROWS + 1 : 0, 0x7fffffff, 0};
       a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
-      if (cache->dtype == B200_BF16) rc = big ? simt_launch<bf16, 2>(ctx, a) : simt_launch<bf16, 1>(ctx, a);
-      else rc = big ? simt_launch<float, 2>(ctx, a) : simt_launch<float, 1>(ctx, a);
+      rc = cache->dtype == B200_BF16 ? simt_launch<bf16>(ctx, a) : simt_launch<float>(ctx, a);
     }
     if (rc) return rc;
     if (!few) return paged_join_launch(ctx, a, nullptr, cache->dtype);
