@@ -84,7 +84,12 @@ paged_attn_few_kernel(PagedAttnArgs a) {
         cp_async16(d, (const bf16 *)a.k + e, o >= 0);
         cp_async16(d + HALF, (const bf16 *)a.v + e, o >= 0);
       }
-      if (++ld_kt >= ld.k1) { ld.next(a.b, a.plan, run.end); ld_kt = 0; }
+      if (++ld_kt >= ld.k1) {
+        ld.next(a.b, a.plan, run.end); ld_kt = 0;
+        // the next block's queries come nearer while the ring still holds keys of this one
+        if (ld.more && warp == 0 && lane * 64 < a.plan.G * HD)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"((const bf16 *)a.q + (size_t)ld.pl.q.q0 * a.ld_q + (size_t)ld.pl.kvh * a.plan.G * HD + lane * 64));
+      }
       page = fetch_page();
     }
     cp_commit();
@@ -210,21 +215,26 @@ paged_attn_few_kernel(PagedAttnArgs a) {
         const float top = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
         f[h] = top == -INFINITY ? 0.f : ex2(mx[m][h] - top);
       }
-      for (int x = 0; x < WARPS; ++x) {
-        if (warp == x) {
+      // blocks of up to 8 (4) rows leave room for two (four) warps' parts side by side, and take as many rounds less
+      const int n_rows = min(16, pl.q.ql * a.plan.G - m * 16), side = n_rows <= 4 ? 4 : n_rows <= 8 ? 2 : 1, part = 16 / side;
+      for (int x = 0; x < WARPS; x += side) {
+        if (warp / side == x / side) {
+          float *mine = sO + (warp % side) * part * OST;
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int h = 0; h < 2; ++h)
+            if (g + 8 * h < part) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float2 *d = (float2 *)(sO + (g + 8 * h) * OST + n * 8 + t4 * 2);
-              float2 y = x ? *d : make_float2(0.f, 0.f);
-              y.x = fmaf(o[m][n][2 * h], f[h], y.x); y.y = fmaf(o[m][n][2 * h + 1], f[h], y.y);
-              *d = y;
+              for (int n = 0; n < NT; ++n) {
+                float2 *d = (float2 *)(mine + (g + 8 * h) * OST + n * 8 + t4 * 2);
+                float2 y = x ? *d : make_float2(0.f, 0.f);
+                y.x = fmaf(o[m][n][2 * h], f[h], y.x); y.y = fmaf(o[m][n][2 * h + 1], f[h], y.y);
+                *d = y;
+              }
             }
         }
         __syncthreads();
       }
-      for (int i = tid; i < 16 * CH; i += THREADS) {
+      for (int i = tid; i < n_rows * CH; i += THREADS) {
         const int r = m * 16 + i / CH, d = (i % CH) * 8;
         int row, head, pos;
         if (!paged_row(a, pl, r, row, head, pos)) continue;
@@ -234,6 +244,10 @@ paged_attn_few_kernel(PagedAttnArgs a) {
         for (int x = 0; x < WARPS; ++x) sum = fmaf(sm_l[x][r], ex2(sm_m[x][r] - base), sum);
         const float *src = sO + (r & 15) * OST + d;
         float4 y0 = *(const float4 *)src, y1 = *(const float4 *)(src + 4);
+        for (int x = 1; x < side; ++x) {
+          const float4 z0 = *(const float4 *)(src + x * part * OST), z1 = *(const float4 *)(src + x * part * OST + 4);
+          y0.x += z0.x; y0.y += z0.y; y0.z += z0.z; y0.w += z0.w; y1.x += z1.x; y1.y += z1.y; y1.z += z1.z; y1.w += z1.w;
+        }
         if (whole) {
           const float inv = sum > 0.f ? 1.0f / sum : 0.f;
           const uint4 out = make_uint4(pack2(y0.x * inv, y0.y * inv), pack2(y0.z * inv, y0.w * inv), pack2(y1.x * inv, y1.y * inv), pack2(y1.z * inv, y1.w * inv));
@@ -275,7 +289,7 @@ bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t l
 
 int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, bool beside) {
   const bool two = (long long)a.b.max_q * G > 16;
-  a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 2, 0, two ? PAGED_FEW_ROWS : 16, 0};
+  a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 3, 0, two ? PAGED_FEW_ROWS : 16, 0};
   a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1; a.beside = beside ? 1 : 0;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);
   return two ? launch_t<64, 2>(ctx, a) : launch_t<64, 1>(ctx, a);
