@@ -4,18 +4,22 @@
 // on the pairs (2i, 2i + 1) of the interleaved layout or (i, i + rotary_dim / 2) of the half layout; the rest of the head is
 // copied.  The backward pass is the transpose: theta negated.  Extends the dense form of cpp/src/Positional.cpp:120-147.
 //
-// Bound by memory: every element is read once and written once.  One CTA takes a few tokens; it evaluates each (token, pair)
-// angle once into shared memory and uses it for all heads, so the angles can be exact: the product with the 64-bit
-// frequency and the reduction to one turn are done in 64 bits (a 32-bit product is off by 6e-3 rad at position 10^5), the
-// sine and cosine of the reduced angle in 32.  Vectors of 16 bytes when alignment and layout allow, else element by element.
-// Appending k and v with the rotation of q and k is one launch: rows go from the projection's output straight to their pages.
+// Bound by memory: every element is read once and written once.  One CTA takes up to four tokens; it evaluates each (token, pair) angle
+// once into shared memory and uses it for all heads, so the angles can be exact: the product with the 64-bit frequency and the
+// reduction to one turn are done in 64 bits (a 32-bit product is off by 6e-3 rad at position 10^5), the sine and cosine of the
+// reduced angle in 32.  Vectors of 16 bytes when alignment and layout allow, else element by element.  What hides the memory's
+// latency is the number of threads: eight CTAs of 256 per SM with one vector each in flight take 36.9 us for the gradients of 16384
+// tokens of 16 + 4 heads of 128 in bf16 (4.55 TB/s); two or four vectors a thread at four to six CTAs took 41 to 51, a form with the
+// angles in registers that walks over the heads (less contiguous) 40 to 47.
+// Appending k and v with the rotation of q and k is one launch: rows go from the projection's output straight to their pages
+// (8892 tokens of 32 + 8 + 8 heads of 128 in bf16: 43.5 us, 5.0 TB/s).
 #include "paged_common.cuh"
 #include <algorithm>
 #include <cmath>
 
 namespace {
 
-constexpr int THREADS = 256, MAX_PAIRS = 512;      // (token, pair) angles in shared memory per CTA
+constexpr int THREADS = 256, MAX_PAIRS = 512, MAX_TOKENS = 8, TOKENS = 4;      // MAX_PAIRS: (token, pair) angles in shared memory per CTA
 
 struct RopeArgs {
   const double *freqs;
@@ -28,69 +32,71 @@ struct RopeArgs {
   int paged;
 };
 
-// One 16-byte vector (or one element) of a head: which elements it holds is fixed by `item`.
-template <class T, bool HALF, bool VEC>
-__device__ __forceinline__ void turn(const T *src, T *dst, int item, int rd, const float2 *cs, bool rotate) {
-  constexpr int N = VEC ? Vec16<T>::N : 1;
-  if constexpr (VEC) {
-    if (!rotate) { reinterpret_cast<uint4 *>(dst)[item] = reinterpret_cast<const uint4 *>(src)[item]; return; }
+// A rotated vector of a head: its 16 bytes (interleaved layout, or the copied rest), or the two that pair (half layout).  The sines and cosines
+// of an item are float4 (two pairs each) `stride` apart, so that the items of a warp read neighbouring ones.
+template <class T, bool HALF>
+struct Piece {
+  static constexpr int N = Vec16<T>::N, PAIRS = HALF ? N : N / 2, QUADS = PAIRS / 2;
+  Vec16<T> x, y;
+  __device__ __forceinline__ void load(const T *src, int item, int turned) {
     if constexpr (HALF) {
-      const int units = rd / 2 / N;                // vector pairs, then the copied rest
-      if (item >= units) { reinterpret_cast<uint4 *>(dst)[item + units] = reinterpret_cast<const uint4 *>(src)[item + units]; return; }
-      Vec16<T> x, y;
-      float a[N], b[N];
-      x.load(src + item * N); y.load(src + rd / 2 + item * N);
-      x.unpack(a); y.unpack(b);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float2 c = cs[item * N + j];
-        const float u = a[j] * c.x - b[j] * c.y, w = a[j] * c.y + b[j] * c.x;
-        a[j] = u; b[j] = w;
-      }
-      x.pack(a); y.pack(b);
-      x.store(dst + item * N); y.store(dst + rd / 2 + item * N);
-    } else {
-      if (item * N >= rd) { reinterpret_cast<uint4 *>(dst)[item] = reinterpret_cast<const uint4 *>(src)[item]; return; }
-      Vec16<T> x;
-      float a[N];
-      x.load(src + item * N); x.unpack(a);
-#pragma unroll
-      for (int j = 0; j < N / 2; ++j) {
-        const float2 c = cs[item * (N / 2) + j];
-        const float u = a[2 * j] * c.x - a[2 * j + 1] * c.y, w = a[2 * j] * c.y + a[2 * j + 1] * c.x;
-        a[2 * j] = u; a[2 * j + 1] = w;
-      }
-      x.pack(a); x.store(dst + item * N);
-    }
-  } else {
-    if (!rotate) { dst[item] = src[item]; return; }
-    if (item >= rd / 2) { dst[item + rd / 2] = src[item + rd / 2]; return; }
-    const int i = HALF ? item : 2 * item, j = HALF ? item + rd / 2 : 2 * item + 1;
-    const float a = to_f(src[i]), b = to_f(src[j]);
-    const float2 c = cs[item];
-    dst[i] = from_f<T>(a * c.x - b * c.y); dst[j] = from_f<T>(a * c.y + b * c.x);
+      if (item < turned) { x.load(src + item * N); y.load(src + (item + turned) * N); }
+      else x.load(src + (item + turned) * N);
+    } else x.load(src + item * N);
   }
+  __device__ __forceinline__ void turn_store(T *dst, int item, int turned, const float4 *cs, int stride) {
+    if (item >= turned) { x.store(dst + (HALF ? item + turned : item) * N); return; }
+    float a[N], b[N];
+    x.unpack(a);
+    if constexpr (HALF) y.unpack(b);
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) {
+      const float4 q = cs[k * stride];
+      const float2 c[2] = {make_float2(q.x, q.y), make_float2(q.z, q.w)};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int p = 2 * k + j;
+        float &u = HALF ? a[p] : a[2 * p], &w = HALF ? b[p] : a[2 * p + 1];
+        const float u0 = u, w0 = w;
+        u = u0 * c[j].x - w0 * c[j].y; w = u0 * c[j].y + w0 * c[j].x;
+      }
+    }
+    x.pack(a); x.store(dst + item * N);
+    if constexpr (HALF) { y.pack(b); y.store(dst + (item + turned) * N); }
+  }
+};
+// element by element: a pair, then the copied rest
+template <class T, bool HALF>
+__device__ __forceinline__ void turn_one(const T *src, T *dst, int item, int rd, const float2 *cs) {
+  if (item >= rd / 2) { dst[item + rd / 2] = src[item + rd / 2]; return; }
+  const int i = HALF ? item : 2 * item, j = HALF ? item + rd / 2 : 2 * item + 1;
+  const float a = to_f(src[i]), b = to_f(src[j]);
+  const float2 c = cs[item];
+  dst[i] = from_f<T>(a * c.x - b * c.y); dst[j] = from_f<T>(a * c.y + b * c.x);
 }
 
 template <class T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 8)
 rope_positions_kernel(RopeArgs r, PagedArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int N = VEC ? Vec16<T>::N : 1;
-  __shared__ float2 cs[MAX_PAIRS];
-  __shared__ int pos_s[MAX_PAIRS];
-  __shared__ long long slot_s[MAX_PAIRS];              // element offset of the row's slot in the pages; -1: no slot
+  typedef Piece<T, HALF> P;
+  constexpr int N = P::N;
+  __shared__ float4 cs4[MAX_PAIRS / 2];
+  __shared__ int pos_s[MAX_TOKENS];
+  __shared__ long long slot_s[MAX_TOKENS];             // element offset of the row's slot in the pages; -1: no slot, -2: no sequence
+  float2 *cs = reinterpret_cast<float2 *>(cs4);
   const int t0 = blockIdx.x * r.per_cta, nt = min(r.per_cta, r.tokens - t0), pairs = r.rd / 2, tid = threadIdx.x;
+  const int H = r.qh + r.kvh, rows = nt * H, turned = VEC ? pairs / P::PAIRS : pairs;      // rows to rotate: a token's query heads, then its key heads
   if (r.paged) {
-    for (int t = tid; t < nt; t += THREADS) slot_s[t] = -2;     // behind the last sequence: left as it is
+    for (int t = tid; t < nt; t += THREADS) slot_s[t] = -2;
     __syncthreads();
     for (int s = tid; s < a.n_seq; s += THREADS) {
       const paged::Seq q = paged::load_seq(a, s);
       const int lo = max(q.q0, t0), hi = min(q.q0 + q.ql, t0 + nt);
       for (int t = lo; t < hi; ++t) {
         const int pos = q.base + (t - q.q0);
-        long long slot = -1;                                      // rows before the first position are padding
+        long long slot = -1;                           // rows before the first position are padding
         if (pos >= 0) {
           const int page = paged::page_of(a, s, pos);
           if (page >= 0) slot = (long long)page * a.page_stride + (long long)(pos % a.page_size) * a.token_stride;
@@ -101,41 +107,78 @@ rope_positions_kernel(RopeArgs r, PagedArgs a) {
     __syncthreads();
   }
   for (int i = tid; i < nt * pairs; i += THREADS) {
-    const int t = i / pairs;
+    const int t = i / pairs, p = i - t * pairs;
     if (r.paged && slot_s[t] == -2) continue;
-    const double turns = (double)(r.paged ? pos_s[t] : r.positions[t0 + t]) * (r.freqs[i - t * pairs] * 0.15915494309189533577);
+    const double turns = (double)(r.paged ? pos_s[t] : r.positions[t0 + t]) * (r.freqs[p] * 0.15915494309189533577);
     float sn, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &sn, &c);
-    cs[i] = make_float2(c * r.amplitude, sn * r.amplitude * r.sign);
+    int at = i;
+    if constexpr (VEC) { const int item = p / P::PAIRS, j = p % P::PAIRS; at = ((t * P::QUADS + j / 2) * turned + item) * 2 + (j & 1); }
+    cs[at] = make_float2(c * r.amplitude, sn * r.amplitude * r.sign);
   }
   __syncthreads();
-  const int turned = VEC ? (HALF ? r.hd / N - pairs / N : r.hd / N) : r.hd - pairs;    // items of a rotated head
-  const int copied = r.hd / N;                                                          // items of a copied one
-  const int nq = r.q ? r.qh * turned : 0, nk = r.kvh * turned, nv = r.v ? r.kvh * copied : 0, per_token = nq + nk + nv;
-  for (int i = tid; i < nt * per_token; i += THREADS) {
-    const int t = i / per_token;
-    int x = i - t * per_token;
+  auto source = [&](int t, int h) -> const T * {
     const size_t row = (size_t)t0 + t;
-    if (r.paged && slot_s[t] == -2) continue;
-    const float2 *c = cs + t * pairs;
-    if (x < nq) {
-      const int h = x / turned;
-      turn<T, HALF, VEC>((const T *)r.q + row * r.ld_q + (size_t)h * r.hd, (T *)r.q_out + row * r.ld_qo + (size_t)h * r.hd, x - h * turned, r.rd, c, pairs > 0);
-      continue;
+    return h < r.qh ? (const T *)r.q + row * r.ld_q + (size_t)h * r.hd : (const T *)r.k + row * r.ld_k + (size_t)(h - r.qh) * r.hd;
+  };
+  auto target = [&](int t, int h) -> T * {             // null: the row is left as it is
+    const size_t row = (size_t)t0 + t;
+    if (h < r.qh) return r.paged && slot_s[t] == -2 ? nullptr : (T *)r.q_out + row * r.ld_qo + (size_t)h * r.hd;
+    if (r.paged) return slot_s[t] < 0 ? nullptr : (T *)r.k_out + slot_s[t] + (long long)(h - r.qh) * a.head_stride;
+    return (T *)r.k_out + row * r.ld_ko + (size_t)(h - r.qh) * r.hd;
+  };
+  if constexpr (VEC) {
+    // a thread keeps its place in the head and takes rows one pass of the CTA apart
+    const int items = HALF ? r.hd / N - turned : r.hd / N, pass = THREADS / items, item = tid % items, first = tid / items;
+    if (first < pass) {
+      const int dt = pass / H, dh = pass - dt * H;
+      int t = first / H, h = first - t * H;
+      while (t < nt) {
+        T *dst = target(t, h);
+        if (dst) {
+          P piece;
+          piece.load(source(t, h), item, turned);
+          piece.turn_store(dst, item, turned, cs4 + t * P::QUADS * turned + item, turned);
+        }
+        t += dt; h += dh;
+        if (h >= H) { h -= H; ++t; }
+      }
     }
-    x -= nq;
-    const bool is_k = x < nk;
-    if (!is_k) x -= nk;
-    const int items = is_k ? turned : copied, h = x / items;
-    const T *src = is_k ? (const T *)r.k + row * r.ld_k : (const T *)r.v + row * r.ld_v;
-    T *dst;
-    if (r.paged) {
-      if (slot_s[t] < 0) continue;
-      dst = (T *)(is_k ? r.k_out : r.v_out) + slot_s[t] + (long long)h * a.head_stride;
-    } else {
-      dst = (T *)r.k_out + row * r.ld_ko + (size_t)h * r.hd;
+  } else {
+    const int per_row = r.hd - pairs;
+    for (int i = tid; i < rows * per_row; i += THREADS) {
+      const int x = i / per_row, t = x / H;
+      T *dst = target(t, x - t * H);
+      if (dst) turn_one<T, HALF>(source(t, x - t * H), dst, i - x * per_row, r.rd, cs + t * pairs);
     }
-    turn<T, HALF, VEC>(src + (size_t)h * r.hd, dst, x - h * items, r.rd, c, is_k && pairs > 0);
+  }
+  if (r.v) {                                           // values are copied to their slots
+    const int per_row = VEC ? r.hd / N : r.hd, all = nt * r.kvh * per_row;
+    constexpr int U = VEC ? 4 : 1;
+    for (int i0 = tid; i0 < all; i0 += U * THREADS) {
+      uint4 v[U];
+      T one = from_f<T>(0.f);
+      long long at[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * THREADS;
+        at[j] = -1;
+        if (i < all) {
+          const int x = i / per_row, d = i - x * per_row, t = x / r.kvh, h = x - t * r.kvh;
+          const T *src = (const T *)r.v + ((size_t)t0 + t) * r.ld_v + (size_t)h * r.hd + (VEC ? d * N : d);
+          if (slot_s[t] >= 0) at[j] = slot_s[t] + (long long)h * a.head_stride + (VEC ? d * N : d);
+          if constexpr (VEC) v[j] = *reinterpret_cast<const uint4 *>(src);
+          else one = *src;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (at[j] >= 0) {
+          T *dst = (T *)r.v_out + at[j];
+          if constexpr (VEC) *reinterpret_cast<uint4 *>(dst) = v[j];
+          else *dst = one;
+        }
+    }
   }
 }
 
@@ -185,7 +228,7 @@ int launch(b200_ctx *ctx, RopeArgs &r, const PagedArgs &a, bool half, b200_dtype
   const bool vec = ptrs % 16 == 0 && lds % n == 0 && (size_t)r.hd % n == 0 && (half ? (size_t)(r.rd / 2) % n == 0 : (size_t)r.rd % n == 0);
   // tokens per CTA: as many as their angles fit, while the grid still covers the SMs several times
   const int fit = r.rd ? std::max(1, MAX_PAIRS / (r.rd / 2)) : 8;
-  r.per_cta = std::max(1, std::min(std::min(fit, 4), r.tokens / (4 * ctx->sm_count)));
+  r.per_cta = std::max(1, std::min(std::min(fit, TOKENS), r.tokens / (4 * ctx->sm_count)));
   if (dt == B200_BF16) return half ? launch_t<bf16, true>(ctx, r, a, vec) : launch_t<bf16, false>(ctx, r, a, vec);
   return half ? launch_t<float, true>(ctx, r, a, vec) : launch_t<float, false>(ctx, r, a, vec);
 }
