@@ -225,7 +225,9 @@ int b200_paged_append(b200_ctx *ctx, const b200_paged_cache *cache, const b200_p
                       size_t ld_q_out, size_t q_heads);
 /* Causal attention of the new rows over the cache (which holds them already): o [rows, n_heads, head_dim] and, optional, lse fp32
  * [rows, n_heads], the log-sum-exp of the scaled scores.  scale 0: 1/sqrt(head_dim).  Rows that see nothing get o = 0, lse = -inf.
- * Positions from kv_len on are never used, whatever their slots hold.  head_dim up to 256.
+ * Positions from kv_len on are never used, whatever their slots hold; values inside must be finite.  head_dim up to 256.  o must not
+ * overlap q.  Fast paths: bf16, head_dim 64 or 128, 16-byte aligned rows, for chunks also a page_size that is a multiple of 8 and at most 128
+ * query heads per KV head; everything else runs on CUDA cores.
  * The workspace is the caller's: calls that may overlap, captured graphs among them, each need their own. */
 int b200_paged_attn_workspace(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, size_t n_heads, size_t *bytes);
 int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, const void *q, size_t ld_q, void *o,
@@ -368,7 +370,7 @@ int b200_sample(b200_ctx *ctx, const void *logits, b200_dtype dtype, size_t batc
 /* One sampling step from given random numbers, with settings per row: device arrays of `batch` values, each optional but uniform.
  * logits [batch, vocab] with row stride ld.  Ids are ordered by logit, equal logits by id (lowest first); -inf and NaN logits are
  * masked ids.  With w_i = exp((l_i - max l) / temperature), in 64 bits:
- *   temperature <= 0 or NaN: the first id (the others are not looked at);
+ *   temperature <= 0 or NaN: the first id (the others are not looked at); temperatures above 2^100 count as 2^100;
  *   top_k in 1 .. vocab-1: the first top_k ids stay;    top_p < 1: of these, an id stays while the weight before it is below
  *   top_p x their weight (the first always);            min_p > 0: ids with w_i < min(min_p, 1) go.
  * The token is the lowest id that stays whose cumulative weight, in id order, exceeds uniform x the weight of all that stay; uniform is

@@ -82,6 +82,8 @@ class PagedCache:
         n, p, h, d = k.shape
         if tuple(v.shape) != (n, p, h, d) or v.dtype != k.dtype:
             raise B200Error("k and v pages must be alike")
+        if k.dtype not in ("f32", "bf16"):
+            raise B200Error("pages are f32 or bf16")
         self.k, self.v = k, v
         self.struct = _PagedCache(k.ptr, v.ptr, n, p, h, d, p * h * d if page_stride is None else page_stride,
                                   h * d if token_stride is None else token_stride, d if head_stride is None else head_stride, k.code)
@@ -95,6 +97,8 @@ class PagedBatch:
         n, m = page_table.shape
         if kv_len.size != n or q_start.size != n + 1:
             raise B200Error("q_start, kv_len and page_table must agree on the number of sequences")
+        if any(x.dtype != "i32" for x in (q_start, kv_len, page_table)):
+            raise B200Error("q_start, kv_len and page_table are int32 arrays")
         self.arrays = (q_start, kv_len, page_table)
         self.struct = _PagedBatch(q_start.ptr, kv_len.ptr, page_table.ptr, n, m, rows, max_q)
         self.ref = C.byref(self.struct)
@@ -418,6 +422,8 @@ class Context:
         hd = a.shape[2]
         if hd != cfg.head_dim or positions.size != a.shape[0] or (q is not None and k is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0] or k.shape[2] != hd)):
             raise B200Error("rope_positions: q [tokens, heads, head_dim], k and positions must agree")
+        if a.dtype not in ("f32", "bf16") or positions.dtype != "i32" or (freqs is not None and (freqs.dtype != "f64" or freqs.size < cfg.rotary_dim // 2)):
+            raise B200Error("rope_positions: f32 or bf16 rows, i32 positions, f64 frequencies [rotary_dim / 2]")
         for x, y in ((q, qo), (k, ko)):
             if x is not None and (y is None or y.shape != x.shape or y.dtype != x.dtype):
                 raise B200Error("rope_positions: outputs must be like the inputs")
@@ -492,6 +498,8 @@ class Context:
         if (v.shape != k.shape or v.dtype != k.dtype or k.dtype != cache.k.dtype or rows != batch.struct.rows or n != st.n_kv or hd != st.head_dim or
                 (q is not None and (q.shape[0] != rows or q.shape[2] != hd or q.dtype != k.dtype))):
             raise B200Error("paged_append: k, v and q must match the cache and the batch")
+        if freqs is not None and (freqs.dtype != "f64" or (rope is not None and freqs.size < rope.rotary_dim // 2)):
+            raise B200Error("paged_append: f64 frequencies [rotary_dim / 2]")
         if q is not None and q_out is None:
             q_out = self.empty(q.shape, q.dtype)
         elif q is not None and (q_out.shape != q.shape or q_out.dtype != q.dtype):
@@ -584,6 +592,8 @@ class Context:
     def sample_given(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
         """One sampling step from given random numbers with settings per row (device arrays [batch]); returns (tokens, kept, prob)."""
         B, V = logits.shape
+        if logits.dtype not in ("f32", "bf16"):
+            raise B200Error("sample_given: f32 or bf16 logits")
         tok, kept, prob = out if out is not None else (self.empty((B,), "i32"), self.empty((B,), "i32"), self.empty((B,), "f32"))
         for x, t in ((uniform, "f32"), (temperature, "f32"), (top_k, "i32"), (top_p, "f32"), (min_p, "f32"), (tok, "i32"), (kept, "i32"), (prob, "f32")):
             if x is not None and (x.size != B or x.dtype != t):

@@ -7,8 +7,9 @@
 //
 // The CUDA-core kernel: blocks of 32 rows (token, query head of the group) x tiles of 32 keys, one pass with a running
 // maximum and sum.  Warp w owns rows w, w + 4, ...; in the scores a lane is a key, in the product with V four dimensions.
-// Keys and values pass through shared memory in 32 bits.  Bound by shared-memory reads (12 per 32 multiply-adds of a warp
-// with all its rows, fewer instructions with few rows).
+// Keys and values pass through shared memory in 32 bits, four vectors of a thread in flight on the way there.  Bound by shared-memory reads (12 per 32
+// multiply-adds of a warp with all its rows, fewer instructions with few rows); in small calls by the chain of loads, scores and joins
+// (drafts of 14 tokens over seven sequences, 8 query and 2 KV heads of 64 in 32 bits: 25 us).
 #include "paged_attn.cuh"
 #include <algorithm>
 #include <atomic>

@@ -13,6 +13,10 @@
 //     partial result for the join;
 //   * a block with rows for one tile only (up to 128: a short chunk, the end of a long one) gives both tiles the same rows and alternate key
 //     tiles, so that the two still alternate on the tensor pipe; their results are joined through shared memory at the end.
+// 1024 tokens over 30011 positions, 32 query and 8 KV heads of 128: 485 us by itself (1.02 PFLOP/s), 600 us in a loop of its own at the power limit
+// (0.82 PFLOP/s, half the matrix rate).  A key tile takes 2.3 to 2.5 us for 256 rows in long runs; a block's start and end about 10 us, which
+// is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us): the boxes of
+// small pages already fill the copy engine's issue rate.
 // Tensor memory: [S_A 128 | O_A 128 | S_B 128 | O_B 128] columns.  Warps 0-3 softmax of tile A, 4-7 of tile B, 8 MMA issue, 9 loads, 10 value rows.
 #include "attention_tc.cuh"
 #include "paged_attn.cuh"
@@ -475,6 +479,7 @@ bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const vo
 }
 
 int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, int min_rows) {
+  // a tile costs two units, one where only one row tile has rows (it then takes half the time); a block's start and end six
   a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 6, min_rows, 0x7fffffff, 1};
   a.n_cta = ctx->sm_count; a.min_units = 4; a.slot_rows = 256; a.vec_out = 1; a.beside = 0;
   return a.b.hd == 128 ? launch_t<128>(ctx, a) : launch_t<64>(ctx, a);

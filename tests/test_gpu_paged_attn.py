@@ -76,6 +76,7 @@ LENS = {
     "drafts": ([2, 5, 1, 8], [2, 100, 257, 1000]),
     "padding rows first": ([6, 3], [4, 3]),
     "chunks": ([40, 129], [40, 500]),
+    "long padding": ([100, 40, 3], [60, 0, 0]),
     "chunks and tokens": ([1, 150, 1, 1, 33], [700, 150, 5, 1200, 90]),
 }
 HEADS = [(4, 1, 128), (8, 2, 64), (3, 3, 128), (5, 1, 64), (16, 2, 128), (6, 2, 80), (2, 1, 256), (3, 1, 20)]
@@ -170,6 +171,43 @@ def test_shared_prefix_pages(ctx, dtype):
     m.batch = bridge.PagedBatch(ctx.array(m.q_start, "i32"), ctx.array(np.array(m.kv_lens, np.int32), "i32"), ctx.array(m.table, "i32"), m.rows)
     run(ctx, m)
     m.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [([1], [1000]), ([2, 1], [40, 3000]), ([200], [700])])
+def test_without_a_bound_on_the_rows_of_a_sequence(ctx, lens, dtype):
+    """max_q 0 stands for all rows, of which there are many more than the sequences use."""
+    m = Made(ctx, *lens, 8, 2, 128, 16, dtype, spare=150)
+    m.batch = bridge.PagedBatch(*m.batch.arrays, m.rows)
+    run(ctx, m)
+    m.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_sequence_longer_than_the_bound_is_reported(ctx, dtype):
+    m = Made(ctx, [1, 60], [100, 100], 8, 2, 64, 16, dtype)
+    m.batch = bridge.PagedBatch(*m.batch.arrays, m.rows, 50)
+    with pytest.raises(bridge.B200Error, match="paged batch"):
+        run(ctx, m)
+    m.batch = bridge.PagedBatch(*m.batch.arrays, m.rows, 60)
+    run(ctx, m)
+    m.check()
+
+
+def test_arrays_of_the_wrong_kind_are_refused(ctx):
+    m = Made(ctx, [1], [5], 4, 1, 64, 16, "f32")
+    with pytest.raises(bridge.B200Error, match="int32"):
+        bridge.PagedBatch(ctx.array(m.q_start.astype(np.float32)), *m.batch.arrays[1:], m.rows)
+    with pytest.raises(bridge.B200Error, match="f32 or bf16"):
+        bridge.PagedCache(ctx.empty((2, 16, 1, 64), "f64"), ctx.empty((2, 16, 1, 64), "f64"))
+    for bad in (dict(q=ctx.empty((3, 4, 64), "bf16")), dict(out=ctx.empty((3, 4, 32))), dict(lse=ctx.empty((3, 5)))):
+        kw = {**dict(q=m.d_q, out=m.out, lse=m.lse), **bad}
+        with pytest.raises(bridge.B200Error):
+            ctx.paged_attn(m.cache, m.batch, **kw)
+    with pytest.raises(bridge.B200Error):
+        ctx.rope_positions_forward(bridge.RopeConfig.make(64), ctx.empty((32,), "f32"), ctx.empty((3,), "i32"), m.d_q)
+    with pytest.raises(bridge.B200Error):
+        ctx.sample_given(ctx.empty((3, 8), "i32"), ctx.empty((3,)))
 
 
 def test_empty_batches_are_no_work(ctx):
