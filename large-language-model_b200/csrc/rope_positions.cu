@@ -8,11 +8,11 @@
 // once into shared memory and uses it for all heads, so the angles can be exact: the product with the 64-bit frequency and the
 // reduction to one turn are done in 64 bits (a 32-bit product is off by 6e-3 rad at position 10^5), the sine and cosine of the
 // reduced angle in 32.  Vectors of 16 bytes when alignment and layout allow, else element by element.  What hides the memory's
-// latency is the number of threads: eight CTAs of 256 per SM with one vector each in flight take 36.9 us for the gradients of 16384
-// tokens of 16 + 4 heads of 128 in bf16 (4.55 TB/s); two or four vectors a thread at four to six CTAs took 41 to 51, a form with the
+// latency is the number of threads: eight CTAs of 256 per SM with one vector each in flight take 34.9 us for the gradients of 16384
+// tokens of 16 + 4 heads of 128 in bf16 (4.8 TB/s); two or four vectors a thread at four to six CTAs took 41 to 51, a form with the
 // angles in registers that walks over the heads (less contiguous) 40 to 47.
 // Appending k and v with the rotation of q and k is one launch: rows go from the projection's output straight to their pages
-// (8892 tokens of 32 + 8 + 8 heads of 128 in bf16: 43.5 us, 5.0 TB/s).
+// (8892 tokens of 32 + 8 + 8 heads of 128 in bf16: 43.2 us, 5.1 TB/s).
 #include "paged_common.cuh"
 #include <algorithm>
 #include <cmath>
@@ -32,6 +32,23 @@ struct RopeArgs {
   int paged;
 };
 
+// Two bf16 values at a time where the type allows.
+template <class T> __device__ __forceinline__ void unpack16(const Vec16<T> &v, float *f) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w[4] = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  } else v.unpack(f);
+}
+template <class T> __device__ __forceinline__ void pack16(Vec16<T> &v, const float *f) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&h); }
+    v.raw = make_uint4(w[0], w[1], w[2], w[3]);
+  } else v.pack(f);
+}
+
 // A rotated vector of a head: its 16 bytes (interleaved layout, or the copied rest), or the two that pair (half layout).  The sines and cosines
 // of an item are float4 (two pairs each) `stride` apart, so that the items of a warp read neighbouring ones.
 template <class T, bool HALF>
@@ -47,8 +64,8 @@ struct Piece {
   __device__ __forceinline__ void turn_store(T *dst, int item, int turned, const float4 *cs, int stride) {
     if (item >= turned) { x.store(dst + (HALF ? item + turned : item) * N); return; }
     float a[N], b[N];
-    x.unpack(a);
-    if constexpr (HALF) y.unpack(b);
+    unpack16(x, a);
+    if constexpr (HALF) unpack16(y, b);
 #pragma unroll
     for (int k = 0; k < QUADS; ++k) {
       const float4 q = cs[k * stride];
@@ -61,8 +78,8 @@ struct Piece {
         u = u0 * c[j].x - w0 * c[j].y; w = u0 * c[j].y + w0 * c[j].x;
       }
     }
-    x.pack(a); x.store(dst + item * N);
-    if constexpr (HALF) { y.pack(b); y.store(dst + (item + turned) * N); }
+    pack16(x, a); x.store(dst + item * N);
+    if constexpr (HALF) { pack16(y, b); y.store(dst + (item + turned) * N); }
   }
 };
 // element by element: a pair, then the copied rest
@@ -75,7 +92,8 @@ __device__ __forceinline__ void turn_one(const T *src, T *dst, int item, int rd,
   dst[i] = from_f<T>(a * c.x - b * c.y); dst[j] = from_f<T>(a * c.y + b * c.x);
 }
 
-template <class T, bool HALF, bool VEC>
+// Off: the type of element offsets into q and k, 32 bits where the arrays are that small (a fifth of the instructions is address arithmetic otherwise).
+template <class T, bool HALF, bool VEC, class Off>
 __global__ void __launch_bounds__(THREADS, 8)
 rope_positions_kernel(RopeArgs r, PagedArgs a) {
   pdl_launch_dependents();
@@ -118,14 +136,14 @@ rope_positions_kernel(RopeArgs r, PagedArgs a) {
   }
   __syncthreads();
   auto source = [&](int t, int h) -> const T * {
-    const size_t row = (size_t)t0 + t;
-    return h < r.qh ? (const T *)r.q + row * r.ld_q + (size_t)h * r.hd : (const T *)r.k + row * r.ld_k + (size_t)(h - r.qh) * r.hd;
+    const Off row = (Off)(t0 + t);
+    return h < r.qh ? (const T *)r.q + (row * (Off)r.ld_q + (Off)(h * r.hd)) : (const T *)r.k + (row * (Off)r.ld_k + (Off)((h - r.qh) * r.hd));
   };
   auto target = [&](int t, int h) -> T * {             // null: the row is left as it is
-    const size_t row = (size_t)t0 + t;
-    if (h < r.qh) return r.paged && slot_s[t] == -2 ? nullptr : (T *)r.q_out + row * r.ld_qo + (size_t)h * r.hd;
+    const Off row = (Off)(t0 + t);
+    if (h < r.qh) return r.paged && slot_s[t] == -2 ? nullptr : (T *)r.q_out + (row * (Off)r.ld_qo + (Off)(h * r.hd));
     if (r.paged) return slot_s[t] < 0 ? nullptr : (T *)r.k_out + slot_s[t] + (long long)(h - r.qh) * a.head_stride;
-    return (T *)r.k_out + row * r.ld_ko + (size_t)(h - r.qh) * r.hd;
+    return (T *)r.k_out + (row * (Off)r.ld_ko + (Off)((h - r.qh) * r.hd));
   };
   if constexpr (VEC) {
     // a thread keeps its place in the head and takes rows one pass of the CTA apart
@@ -215,8 +233,11 @@ int check_config(b200_ctx *ctx, const b200_rope_config *c) {
 template <class T, bool HALF>
 int launch_t(b200_ctx *ctx, const RopeArgs &r, const PagedArgs &a, bool vec) {
   const dim3 grid((unsigned)((r.tokens + r.per_cta - 1) / r.per_cta));
-  if (vec) B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, true>, grid, dim3(THREADS), 0, 0, r, a));
-  else B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, false>, grid, dim3(THREADS), 0, 0, r, a));
+  const unsigned long long most = (unsigned long long)r.tokens * std::max(std::max(r.ld_q, r.ld_qo), std::max(r.ld_k, r.ld_ko));
+  const bool small = (unsigned long long)(r.ld_q | r.ld_qo | r.ld_k | r.ld_ko) < (1ull << 31) && most < (1ull << 32);
+  if (vec && small) B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, true, unsigned>, grid, dim3(THREADS), 0, 0, r, a));
+  else if (vec) B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, true, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
+  else B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, false, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
