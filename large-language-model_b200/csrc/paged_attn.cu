@@ -369,7 +369,7 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
     if (tc) rc = paged_attn_tc_launch(ctx, a, G, few ? PAGED_FEW_ROWS + 1 : 0);
     else {
       a.vec_out = 0; a.beside = 0;
-      a.plan = paged::Plan{G, 0, ROWS, 5, 1, few ? PAGED_FEW_ROWS + 1 : 0, 0x7fffffff, 0};
+      a.plan = paged::Plan{G, 0, ROWS, 5, 1, few ? PAGED_FEW_ROWS + 1 : 0, 0x7fffffff};
       a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
       rc = cache->dtype == B200_BF16 ? simt_launch<bf16>(ctx, a) : simt_launch<float>(ctx, a);
     }
@@ -405,14 +405,14 @@ extern "C" int b200_internal_paged_probe(const b200_paged_cache *cache, const b2
   return B200_OK;
 }
 // Steps through the runs of all CTAs; writes (CTA, sequence, KV head, block, tile, whole block, parts to join at the CTA's border) per tile, returns how many.
-extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile_log2, int extra, int halves,
+extern "C" long long b200_internal_paged_cover(const b200_paged_cache *cache, const b200_paged_batch *batch, int G, int tokens, int rows, int tile_log2, int extra,
                                                int lo, int hi, int n_cta, int min_units, int *out, long long room) {
   int status = 0;
   b200_ctx ctx;
   PagedArgs a;
   if (paged_args(&ctx, cache, batch, &a)) return -1;
   a.status = &status;
-  const paged::Plan p{G, tokens, rows, tile_log2, extra, lo, hi, halves};
+  const paged::Plan p{G, tokens, rows, tile_log2, extra, lo, hi};
   long long total = 0, n_out = 0;
   for (int s = 0; s < a.n_seq; ++s) total += paged::seq_units(a, p, s);
   if (total == 0) return 0;

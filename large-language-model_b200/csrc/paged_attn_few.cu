@@ -294,7 +294,7 @@ int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, bool beside) {
   const bool two = (long long)a.b.max_q * G > 16;
   // extra 3: a block's start and end cost three tiles' time (2: 125 us, 1: 143 us, 4: as 3, at the ragged step above); runs of at least two
   // tiles (1: 17.9 us, 4: 18.9 us, 8: 23.8 us against 14.9 us for the four short sequences)
-  a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 3, 0, two ? PAGED_FEW_ROWS : 16, 0};
+  a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 3, 0, two ? PAGED_FEW_ROWS : 16};
   a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1; a.beside = beside ? 1 : 0;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);
   return two ? launch_t<64, 2>(ctx, a) : launch_t<64, 1>(ctx, a);

@@ -10,12 +10,13 @@
 //     ahead.  Rows behind the sequence's end are boxes out of bounds (zeros) or, inside the last page, whatever was there: scores are
 //     masked, and one warp overwrites those value rows with zeros before the product (0 x NaN is NaN);
 //   * the grid is one CTA per SM, and each walks its equal run of (sequence, KV head, block, key tile): a run that cuts a block leaves a
-//     partial result for the join;
-//   * a block with rows for one tile only (up to 128: a short chunk, the end of a long one) gives both tiles the same rows and alternate key
-//     tiles, so that the two still alternate on the tensor pipe; their results are joined through shared memory at the end.
+//     partial result for the join.
+// A block with rows for one tile only leaves the other idle; giving both alternate key tiles of the same rows was no faster (two buffers
+// of keys and of values then hold no tile ahead: 3.2 thousand cycles a key tile against 4.2, and 6 thousand more to join the two; mixed batch 150 us
+// against 127).
 // 1024 tokens over 30011 positions, 32 query and 8 KV heads of 128: 485 us by itself (1.02 PFLOP/s), 600 us in a loop of its own at the power limit
 // (0.82 PFLOP/s, half the matrix rate).  A key tile takes 2.3 to 2.5 us for 256 rows in long runs; a block's start and end about 10 us, which
-// is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us): the boxes of
+// is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us, before the last two steps): the boxes of
 // small pages already fill the copy engine's issue rate.
 // Tensor memory: [S_A 128 | O_A 128 | S_B 128 | O_B 128] columns.  Warps 0-3 softmax of tile A, 4-7 of tile B, 8 MMA issue, 9 loads, 10 value rows.
 #include "attention_tc.cuh"
@@ -33,7 +34,6 @@ struct alignas(16) TcShared {
   int abort_flag;
   long long red[33];
   paged::Place place;
-  float mix_m[128], mix_l[128];
 };
 
 constexpr float RESCALE_THRESHOLD = 8.0f;      // log2 units: P stays below 2^8
@@ -47,11 +47,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// What a CTA does of one block: key tiles [k0, k1).  Row tile X takes tiles from(X), from(X) + step, .. below end(X): all that its rows see or,
-// where there are no rows for the second (split), every other one.
+// What a CTA does of one block: key tiles [k0, k1); row tile X takes part in those below n[X] (0: it has no rows).
 struct Segment {
-  int k0, k1, n[2], step;
-  bool split;
+  int k0, k1, n[2];
   __device__ __forceinline__ Segment(const PagedAttnArgs &a, const paged::Walk &w) {
     const int half = a.plan.tokens_per_block / 2, t0 = w.pl.block * a.plan.tokens_per_block;
     k0 = w.pl.kt; k1 = w.k1;
@@ -60,11 +58,9 @@ struct Segment {
       const int first = t0 + X * half, last = min(w.pl.q.ql, first + half);          // tokens [first, last)
       n[X] = first < w.pl.q.ql ? max(1, (min(max(w.pl.q.base + last, 0), w.pl.q.len) + TK - 1) / TK) : 0;
     }
-    split = n[1] == 0;
-    step = split ? 2 : 1;
   }
-  __device__ __forceinline__ int from(int X) const { return split ? k0 + X : k0; }
-  __device__ __forceinline__ int end(int X) const { return split ? k1 : max(k0, min(k1, n[X])); }
+  __device__ __forceinline__ int end(int X) const { return max(k0, min(k1, n[X])); }
+  __device__ __forceinline__ bool last_reader(int X) const { return X == 1 || n[1] == 0; }      // B, where it has rows, sees every tile that A sees
   // the value tile with rows behind the sequence's end, or -1
   __device__ __forceinline__ int ragged(const paged::Place &pl) const {
     const int j = pl.q.len / TK;
@@ -81,7 +77,6 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint8_t *sQ = smem, *sK = sQ + 2 * TILE_BYTES, *sV = sK + 2 * TILE_BYTES;
   TcShared *sh = (TcShared *)(sV + 2 * TILE_BYTES);
   uint8_t *stage = (uint8_t *)(sh + 1);          // 8 softmax warps x 2 KiB: transposition buffers of the output stores
-  float4 *mix = (float4 *)(stage + 8 * 2048);    // [8][128] x 16 bytes: 32 columns of the second tile's output on their way to the first
   int *status = a.b.status;
   if (tc::smem_u32(smem) & 1023u) {              // swizzled tiles need 1024-byte alignment: refuse rather than corrupt
     if (threadIdx.x == 0) atomicCAS(status, 0, 298);
@@ -195,9 +190,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             const uint32_t k_addr = tc::smem_u32(sK + s * TILE_BYTES);
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k)
-              tc::umma_ss(tmem_base + X * 256, desc_kmajor(q_addr[g.split ? 0 : X], k), desc_kmajor(k_addr, k), idesc_s, k ? 1u : 0u);
+              tc::umma_ss(tmem_base + X * 256, desc_kmajor(q_addr[X], k), desc_kmajor(k_addr, k), idesc_s, k ? 1u : 0u);
             tc::umma_commit(&sh->s_full[X]);
-            if (X == 1 || g.split) {                       // the tile's last reader (without a split, B sees every tile that A sees)
+            if (g.last_reader(X)) {
               tc::umma_commit(&sh->k_empty[s]);
               if (j == g.k1 - 1) tc::umma_commit(&sh->q_empty);
             }
@@ -215,20 +210,17 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             const uint32_t v_addr = tc::smem_u32(sV + s * TILE_BYTES);
 #pragma unroll
             for (int k = 0; k < TK / 16; ++k)
-              tc::umma_ts(tmem_base + X * 256 + 128, tmem_base + X * 256 + k * 8, desc_mnmajor(v_addr, k), idesc_o, (j >= g.k0 + g.step || k > 0) ? 1u : 0u);
+              tc::umma_ts(tmem_base + X * 256 + 128, tmem_base + X * 256 + k * 8, desc_mnmajor(v_addr, k), idesc_o, (j > g.k0 || k > 0) ? 1u : 0u);
             tc::umma_commit(&sh->o_full[X]);
-            if (X == 1 || g.split) tc::umma_commit(&sh->v_empty[s]);
+            if (g.last_reader(X)) tc::umma_commit(&sh->v_empty[s]);
             ++done[X];
             return true;
           };
-          if (ok && g.from(0) < e[0]) ok = issue_s(0, g.from(0));
-          if (ok && g.from(1) < e[1]) ok = issue_s(1, g.from(1));
+          if (ok && g.k0 < e[0]) ok = issue_s(0, g.k0);
+          if (ok && g.k0 < e[1]) ok = issue_s(1, g.k0);
           for (int j = g.k0; j < g.k1 && ok; ++j) {
-#pragma unroll
-            for (int X = 0; X < 2; ++X) {
-              if (g.split && ((j - g.k0) & 1) != X) continue;
-              if (ok && j < e[X]) { ok = issue_pv(X, j); if (ok && j + g.step < e[X]) ok = issue_s(X, j + g.step); }
-            }
+            if (j < e[0]) { ok = issue_pv(0, j); if (ok && j + 1 < e[0]) ok = issue_s(0, j + 1); }
+            if (ok && j < e[1]) { ok = issue_pv(1, j); if (ok && j + 1 < e[1]) ok = issue_s(1, j + 1); }
           }
           it += g.k1 - g.k0;
           w.next(a.b, a.plan, end);
@@ -264,19 +256,19 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else {
     setmaxnreg_inc<REGS_SOFTMAX>();
     // ---- softmax: warpgroup X owns row tile X, one thread per row
-    const int X = warp >> 2, quarter = warp & 3, lrow = quarter * 32 + lane;
+    const int X = warp >> 2, quarter = warp & 3, r = X * 128 + quarter * 32 + lane;
     const float sl2 = a.scale * PAGED_LOG2E;
     const uint32_t tS = tmem_base + ((uint32_t)(quarter * 32) << 16) + X * 256, tO = tS + 128;
     int cnt = 0;                                           // tiles of this row tile so far
-    while (w.more) {                                       // after a failed wait too: the barriers of split blocks need all eight warps
+    while (w.more && ok) {
       const Segment g(a, w);
-      const int jx = g.end(X), r = (g.split ? 0 : X * 128) + lrow;
+      const int jx = g.end(X);
       int row, head, pos;
       const bool has = paged_row(a, pl, r, row, head, pos);
       const int limit = min(max(pos + 1, 0), pl.q.len);    // keys the row sees
-      const int all_see = min(max(pl.q.base + pl.block * a.plan.tokens_per_block + (r >> 7) * (a.plan.tokens_per_block / 2) + 1, 0), pl.q.len);
+      const int all_see = min(max(pl.q.base + pl.block * a.plan.tokens_per_block + X * (a.plan.tokens_per_block / 2) + 1, 0), pl.q.len);
       float m_used = -1e30f, l = 0.f;                      // a finite start: rows that see nothing stay there with l = 0
-      for (int j = g.from(X); ok && j < jx; j += g.step, ++cnt) {
+      for (int j = g.k0; j < jx; ++j, ++cnt) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh->s_full[X], cnt & 1, status, abort_flag, 270));
         if (!ok) break;                                    // the tensor-memory accesses below are warp-collective
         tc::tc_fence_after();
@@ -300,7 +292,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2);
         const bool need = (m_new - m_used) > RESCALE_THRESHOLD;
-        if (j == g.from(X)) {
+        if (j == g.k0) {
           m_used = m_new;                                  // nothing accumulated yet
         } else if (__any_sync(0xffffffffu, need)) {
           // a row outgrew the maximum in use: rescale its accumulator (the product of the tile before must have landed; this
@@ -339,56 +331,29 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh->p_full[X]);
       }
+      if (!ok) break;
       // ---- the block's end, or the run's: normalised rows, or a partial result
-      const bool whole = w.whole(), any = jx > g.from(X);
-      if (any && ok) {
+      const bool whole = w.whole(), any = jx > g.k0;
+      if (any) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh->o_full[X], (cnt - 1) & 1, status, abort_flag, 272));
+        if (!ok) break;
         tc::tc_fence_after();
-      }
-      // With a split, the second tile hands its maximum and sum, then its output 32 columns at a time, to the first; both take all barriers,
-      // also after a failed wait.
-      float f_own = 1.0f, f_mix = 0.0f;
-      if (g.split) {
-        if (X == 1) { sh->mix_m[lrow] = any && l > 0.f ? m_used : -INFINITY; sh->mix_l[lrow] = any ? l : 0.f; }
-        named_barrier(1, 256);
-        if (X == 0) {
-          const float m2 = sh->mix_m[lrow], l2 = sh->mix_l[lrow], top = fmaxf(l > 0.f ? m_used : -INFINITY, m2);
-          if (top > -INFINITY) { f_own = l > 0.f ? fast_exp2(m_used - top) : 0.f; f_mix = l2 > 0.f ? fast_exp2(m2 - top) : 0.f; m_used = top; l = l * f_own + l2 * f_mix; }
-        }
       }
       const float inv = whole ? (l > 0.f ? 1.0f / l : 0.f) : 1.0f;
       const long long off = !has ? -1 : whole ? (long long)row * a.ld_o + (long long)head * HD : (long long)r * HD;
       float *slot = whole ? nullptr : paged_slot(a, blockIdx.x, g.k0 == 0);
       uint8_t *stg = stage + warp * 2048;
-      const bool writes = g.split ? X == 0 : g.n[X] > 0;
+      const bool writes = g.n[X] > 0;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; writes && c < HD / 32; ++c) {
         uint32_t v[32];
-        if (any && ok) {
+        if (any) {
           tc::tmem_ld_32x32(tO + c * 32, v);
           tc::tmem_ld_wait();
         } else {
 #pragma unroll
           for (int x = 0; x < 32; ++x) v[x] = 0u;
         }
-        if (g.split) {
-          if (X == 1) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) mix[x * 128 + lrow] = make_float4(__uint_as_float(v[4 * x]), __uint_as_float(v[4 * x + 1]), __uint_as_float(v[4 * x + 2]), __uint_as_float(v[4 * x + 3]));
-          }
-          named_barrier(1, 256);
-          if (X == 0) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const float4 y = mix[x * 128 + lrow];
-              const float o[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-              for (int z = 0; z < 4; ++z) v[4 * x + z] = __float_as_uint(__uint_as_float(v[4 * x + z]) * f_own + (f_mix > 0.f ? o[z] * f_mix : 0.f));
-            }
-          }
-          named_barrier(1, 256);
-        }
-        if (!writes || !ok) continue;
         // transposed through a warp-private buffer so that a store instruction writes whole 64-byte pieces of eight rows
         if (whole) {
 #pragma unroll
@@ -427,7 +392,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           }
         }
       }
-      if (ok && writes && has) {
+      if (writes && has) {
         if (!whole) {
           slot[(size_t)256 * HD + r] = l > 0.f ? m_used : -INFINITY;
           slot[(size_t)256 * (HD + 1) + r] = l;
@@ -460,7 +425,7 @@ int launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
       tc_make_map_4d(&mk, a.k, HD, (uint64_t)a.b.page_size, (uint64_t)a.b.n_kv, (uint64_t)a.b.n_pages, (uint64_t)a.b.token_stride * 2, (uint64_t)a.b.head_stride * 2, (uint64_t)a.b.page_stride * 2, 64, (uint32_t)box) ||
       tc_make_map_4d(&mv, a.v, HD, (uint64_t)a.b.page_size, (uint64_t)a.b.n_kv, (uint64_t)a.b.n_pages, (uint64_t)a.b.token_stride * 2, (uint64_t)a.b.head_stride * 2, (uint64_t)a.b.page_stride * 2, 64, (uint32_t)box))
     return b200_fail(ctx, B200_ERR_CUDA, "cuTensorMapEncodeTiled failed for the paged cache");
-  constexpr int smem = 6 * 128 * HD * 2 + (int)sizeof(TcShared) + 8 * 2048 + 128 * 128;
+  constexpr int smem = 6 * 128 * HD * 2 + (int)sizeof(TcShared) + 8 * 2048;
   static_assert(smem <= 232448, "tiles exceed the 227 KiB of shared memory per CTA");
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
@@ -479,8 +444,8 @@ bool paged_attn_tc_supported(const b200_paged_cache *c, size_t n_heads, const vo
 }
 
 int paged_attn_tc_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, int min_rows) {
-  // a tile costs two units, one where only one row tile has rows (it then takes half the time); a block's start and end six
-  a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 6, min_rows, 0x7fffffff, 1};
-  a.n_cta = ctx->sm_count; a.min_units = 4; a.slot_rows = 256; a.vec_out = 1; a.beside = 0;
+  // a block's start and end cost three tiles' time; runs of at least two tiles
+  a.plan = paged::Plan{G, 2 * (128 / G), 0, 7, 3, min_rows, 0x7fffffff};
+  a.n_cta = ctx->sm_count; a.min_units = 2; a.slot_rows = 256; a.vec_out = 1; a.beside = 0;
   return a.b.hd == 128 ? launch_t<128>(ctx, a) : launch_t<64>(ctx, a);
 }

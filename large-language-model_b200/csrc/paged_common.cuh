@@ -69,13 +69,12 @@ __host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int p
 // ---- division of the work ---------------------------------------------------------------------------------------------
 // A sequence's rows (token, query head of the group) are cut into blocks; a block walks the key tiles its last row can see.
 // All (sequence, KV head, block, tile) in this order form one line; a block takes `extra` units (its start and end, in tiles' time)
-// and `cost` per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
+// and one per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
 // whatever the lengths are (without the extra, CTAs whose run held dozens of short sequences took 1.8 times the others' time).
 // A block that crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
 struct Plan {
   int G, tokens_per_block, rows_per_block;   // rows_per_block > 0: blocks of consecutive rows; else blocks of whole tokens
   int tile_log2, extra, min_rows, max_rows;  // keys per tile; only sequences with min_rows <= rows <= max_rows take part
-  int halves;                                // 1: a tile costs two units in blocks with rows in both halves of their tokens, else one
   __host__ __device__ __forceinline__ bool takes(int ql) const { const long long r = (long long)ql * G; return ql > 0 && r >= min_rows && r <= max_rows; }
   __host__ __device__ __forceinline__ int blocks(int ql) const {
     if (max_rows <= rows_per_block) return 1;
@@ -97,11 +96,7 @@ struct Plan {
 };
 // Divisions of positions on the line are 32-bit ones wherever it is that short.
 __host__ __device__ __forceinline__ long long quotient(long long a, int b) { return a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b); }
-// log2 of a tile's cost
-__host__ __device__ __forceinline__ int tile_shift(const Plan &p, const Seq &q, int block) {
-  return p.halves && (long long)block * p.tokens_per_block + p.tokens_per_block / 2 < q.ql ? 1 : 0;
-}
-__host__ __device__ __forceinline__ long long block_units(const Plan &p, const Seq &q, int block) { return ((long long)p.tiles(q, block) << tile_shift(p, q, block)) + p.extra; }
+__host__ __device__ __forceinline__ long long block_units(const Plan &p, const Seq &q, int block) { return (long long)p.tiles(q, block) + p.extra; }
 struct Place { int seq, kvh, block, kt; Seq q; long long first; };   // tile kt of a block, which begins at unit `first`
 
 __host__ __device__ __forceinline__ long long seq_units(const PagedArgs &a, const Plan &p, int s) {
@@ -121,7 +116,7 @@ __host__ __device__ __forceinline__ Place place_in(const PagedArgs &a, const Pla
   int b = 0;
   long long t = block_units(p, pl.q, 0);
   while (u - pl.first >= t) { pl.first += t; t = block_units(p, pl.q, ++b); }
-  pl.block = b; pl.kt = greater(0, (int)(u - pl.first) - p.extra) >> tile_shift(p, pl.q, b);
+  pl.block = b; pl.kt = greater(0, (int)(u - pl.first) - p.extra);
   return pl;
 }
 
@@ -141,8 +136,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long *red, lon
   return before + inc - v;
 }
 
-// CTAs that take part: at most n_max, and few enough that each gets min_units (at least the cost of a tile, so that a run between two
-// others inside a block is never empty).
+// CTAs that take part: at most n_max, and few enough that each gets min_units.
 __host__ __device__ __forceinline__ int line_ctas(long long total, int n_max, int min_units) {
   const long long n = quotient(total, min_units);        // (rounded down: no CTA gets less)
   return n < 1 ? 1 : n < n_max ? (int)n : n_max;
@@ -199,7 +193,7 @@ struct Walk {
   __host__ __device__ __forceinline__ void start(const Plan &p, const Place &at, long long end) { pl = at; set(p, end); }
   __host__ __device__ __forceinline__ void set(const Plan &p, long long end) {
     tiles = p.tiles(pl.q, pl.block);
-    const long long room = (end - pl.first - p.extra) >> tile_shift(p, pl.q, pl.block);      // rounds like the next CTA's start
+    const long long room = end - pl.first - p.extra;
     k1 = room < tiles ? (int)room : tiles;
     more = k1 > pl.kt;                                     // a run that ends in a block's extra leaves it to the next CTA
   }
@@ -224,7 +218,7 @@ struct Walk {
 };
 // How many CTAs, from c - 1 on, have parts of the block that run c begins in; 0 unless c is the first border inside that block.
 __host__ __device__ __forceinline__ int parts_at(const Plan &p, const Run &r, const Place &pl, int c) {
-  if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) >= pl.first + p.extra + (1 << tile_shift(p, pl.q, pl.block))) return 0;
+  if (c == 0 || pl.kt == 0 || line_at(r.total, r.n, c - 1) > pl.first + p.extra) return 0;
   return line_cta(r.total, r.n, pl.first + block_units(p, pl.q, pl.block) - 1) - c + 2;
 }
 

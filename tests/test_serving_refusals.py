@@ -155,13 +155,13 @@ def test_random_tables_stay_inside(lib):
 def cover(lib, q_lens, kv_lens, n_kv, G, few, n_cta, min_units):
     """Every (sequence, KV head, block, tile) that the CTAs' runs visit, by the kernels' own stepping."""
     fn = lib.b200_internal_paged_cover
-    fn.argtypes, fn.restype = [C.c_void_p] * 2 + [C.c_int] * 10 + [C.c_void_p, C.c_longlong], C.c_longlong
+    fn.argtypes, fn.restype = [C.c_void_p] * 2 + [C.c_int] * 9 + [C.c_void_p, C.c_longlong], C.c_longlong
     q_start = np.concatenate(([0], np.cumsum(q_lens))).astype(np.int32)
     kv, table = np.array(kv_lens, np.int32), np.zeros((len(kv_lens), max(1, max(kv_lens))), np.int32)
     c = cache(n_pages=1, page_size=1, n_kv=n_kv, head_dim=1, head_stride=1, token_stride=1, page_stride=1)
     b = bridge._PagedBatch(q_start.ctypes.data, kv.ctypes.data, table.ctypes.data, kv.size, table.shape[1], int(q_start[-1]), 0)
     out = np.empty((200000, 7), np.int32)
-    n = fn(C.byref(c), C.byref(b), G, few["tokens"], few["rows"], int(np.log2(few["tile"])), few["extra"], few["halves"], few["lo"], few["hi"], n_cta, min_units, out.ctypes.data, len(out))
+    n = fn(C.byref(c), C.byref(b), G, few["tokens"], few["rows"], int(np.log2(few["tile"])), few["extra"], few["lo"], few["hi"], n_cta, min_units, out.ctypes.data, len(out))
     assert 0 <= n <= len(out)
     return out[:n]
 
@@ -173,8 +173,8 @@ def test_runs_cover_every_tile_once(lib, seed):
     kv = r.randint(0, 900, n)
     q = np.minimum(np.where(r.rand(n) < 0.5, r.randint(0, 3, n), r.randint(0, 200, n)), kv + 3)
     by_rows = seed % 2
-    plan = dict(extra=int(r.choice([0, 1, 3])), halves=0 if by_rows else int(r.choice([0, 1])), tokens=0 if by_rows else int(r.choice([2, 64, 128])), rows=32 if by_rows else 0, tile=int(r.choice([16, 32, 128])), lo=int(r.choice([0, 17])), hi=int(r.choice([16, 1 << 30])))
-    got = cover(lib, q.tolist(), kv.tolist(), n_kv, G, plan, int(r.choice([1, 5, 148, 296])), int(r.choice([2, 4])))
+    plan = dict(extra=int(r.choice([0, 1, 3])), tokens=0 if by_rows else int(r.choice([2, 64, 128])), rows=32 if by_rows else 0, tile=int(r.choice([16, 32, 128])), lo=int(r.choice([0, 17])), hi=int(r.choice([16, 1 << 30])))
+    got = cover(lib, q.tolist(), kv.tolist(), n_kv, G, plan, int(r.choice([1, 5, 148, 296])), int(r.choice([1, 4])))
     want = set()
     for s in range(n):
         if q[s] == 0 or not plan["lo"] <= q[s] * G <= plan["hi"]:
@@ -191,12 +191,12 @@ def test_runs_cover_every_tile_once(lib, seed):
     cost, blocks, joined = {}, {}, {}
     for ct, sq, h, b, t, whole, parts in got.tolist():
         cost.setdefault(ct, [0, set()])
-        cost[ct][0] += 2 if plan["halves"] and b * plan["tokens"] + plan["tokens"] // 2 < q[sq] else 1
+        cost[ct][0] += 1
         cost[ct][1].add((sq, h, b))
         blocks.setdefault((sq, h, b), []).append((ct, t, whole))
         joined[ct] = parts
     per = [n + plan["extra"] * len(bl) for n, bl in cost.values()]
-    assert not per or max(per) - min(per) <= 2 * plan["extra"] + 3 or len(per) < 2 or max(per) <= -(-sum(per) // len(per)) + 2 * plan["extra"] + 3
+    assert not per or max(per) - min(per) <= 2 * plan["extra"] + 1 or len(per) < 2 or max(per) <= -(-sum(per) // len(per)) + 2 * plan["extra"] + 1
     # a block's CTAs follow each other; the second of them, and no other CTA, joins all of them
     second = {}
     for key, xs in blocks.items():
