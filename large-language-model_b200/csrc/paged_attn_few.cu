@@ -7,9 +7,9 @@
 // Scores and the product with V use m16n8k16 tensor instructions: the 16 (or 32) rows are the padded group of query rows, P goes
 // from accumulators to operand registers without leaving the warp.  Each warp keeps its own running maximum, sum and output; the
 // four are joined through shared memory when a block ends.
-// 64 sequences of 100 to 11865 positions, 32 query and 8 KV heads of 128: 123 us for 665 MB, 5.4 TB/s (82 % of the copy rate; the CUDA-core
+// 64 sequences of 100 to 11865 positions, 32 query and 8 KV heads of 128: 117.5 us for 666 MB, 5.7 TB/s (86 % of the copy rate; the CUDA-core
 // kernel: 4.1 ms).  Most runs end after the 104 us that the memory needs; those that hold many short sequences set the rest.  Four sequences of
-// 200 to 700 positions: 14 us with the join, a chain of latencies (division of the work, keys, scores, joins).
+// 200 to 700 positions: 11.5 us with the join, a chain of latencies (division of the work, keys, scores, joins).
 #include "paged_attn.cuh"
 #include <algorithm>
 #include <atomic>
@@ -273,11 +273,7 @@ int launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
   if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_few_kernel<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr.fetch_or(bit); }
-  const bool pdl = ctx->pdl;
-  ctx->pdl = pdl || a.beside;
-  const cudaError_t e = launch_k(ctx, paged_attn_few_kernel<HD, MT>, dim3((unsigned)a.n_cta), dim3(THREADS), (size_t)smem, 0, a);
-  ctx->pdl = pdl;
-  B200_CUDA(ctx, e);
+  B200_CUDA(ctx, launch_pdl(ctx, paged_attn_few_kernel<HD, MT>, dim3((unsigned)a.n_cta), dim3(THREADS), (size_t)smem, 0, a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
@@ -292,8 +288,8 @@ bool paged_attn_few_supported(const b200_paged_cache *c, const void *q, size_t l
 
 int paged_attn_few_launch(b200_ctx *ctx, PagedAttnArgs &a, int G, bool beside) {
   const bool two = (long long)a.b.max_q * G > 16;
-  // extra 3: a block's start and end cost three tiles' time (2: 125 us, 1: 143 us, 4: as 3, at the ragged step above); runs of at least two
-  // tiles (1: 17.9 us, 4: 18.9 us, 8: 23.8 us against 14.9 us for the four short sequences)
+  // extra 3: a block's start and end cost three tiles' time (against 123 us then, 2: 125, 1: 143, 4: as 3, at the ragged step above); runs of
+  // at least two tiles (against 14.9 us then, 1: 17.9, 4: 18.9, 8: 23.8 for the four short sequences)
   a.plan = paged::Plan{G, 0, two ? 32 : 16, 6, 3, 0, two ? PAGED_FEW_ROWS : 16};
   a.n_cta = 2 * ctx->sm_count; a.min_units = 2; a.slot_rows = two ? 32 : 16; a.vec_out = 1; a.beside = beside ? 1 : 0;
   if (a.b.hd == 128) return two ? launch_t<128, 2>(ctx, a) : launch_t<128, 1>(ctx, a);

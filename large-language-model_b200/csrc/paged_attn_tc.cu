@@ -430,7 +430,7 @@ int launch_t(b200_ctx *ctx, const PagedAttnArgs &a) {
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
   if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(paged_attn_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)); attr.fetch_or(bit); }
-  B200_CUDA(ctx, launch_k(ctx, paged_attn_tc_kernel<HD>, dim3((unsigned)a.n_cta), dim3(TC_THREADS), (size_t)smem, 0, mq, mk, mv, a, box));
+  B200_CUDA(ctx, launch_pdl(ctx, paged_attn_tc_kernel<HD>, dim3((unsigned)a.n_cta), dim3(TC_THREADS), (size_t)smem, 0, mq, mk, mv, a, box));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }

@@ -28,6 +28,17 @@ struct DeviceGuard {                    // entry points may be called with anoth
   ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
+// Programmatic launch whatever the context's setting: these operators are chains of short kernels, each of which waits for the one before in its
+// first instruction (or says why not) and lets the next one launch behind that.
+template <class... K, class... A>
+inline cudaError_t launch_pdl(b200_ctx *ctx, void (*kern)(K...), dim3 grid, dim3 block, size_t smem, int cluster_x, A... args) {
+  const bool pdl = ctx->pdl;
+  ctx->pdl = true;
+  const cudaError_t e = launch_k(ctx, kern, grid, block, smem, cluster_x, args...);
+  ctx->pdl = pdl;
+  return e;
+}
+
 // Host checks of the two descriptors; fills `a`.
 int paged_args(b200_ctx *ctx, const b200_paged_cache *cache, const b200_paged_batch *batch, PagedArgs *a);
 

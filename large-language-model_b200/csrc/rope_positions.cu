@@ -8,11 +8,11 @@
 // once into shared memory and uses it for all heads, so the angles can be exact: the product with the 64-bit frequency and the
 // reduction to one turn are done in 64 bits (a 32-bit product is off by 6e-3 rad at position 10^5), the sine and cosine of the
 // reduced angle in 32.  Vectors of 16 bytes when alignment and layout allow, else element by element.  What hides the memory's
-// latency is the number of threads: eight CTAs of 256 per SM with one vector each in flight take 34.9 us for the gradients of 16384
-// tokens of 16 + 4 heads of 128 in bf16 (4.8 TB/s); two or four vectors a thread at four to six CTAs took 41 to 51, a form with the
+// latency is the number of threads: eight CTAs of 256 per SM with one vector each in flight take 33.2 us for the gradients of 16384
+// tokens of 16 + 4 heads of 128 in bf16 (5.1 TB/s); two or four vectors a thread at four to six CTAs took 41 to 51 where this took 37, a form with the
 // angles in registers that walks over the heads (less contiguous) 40 to 47.
 // Appending k and v with the rotation of q and k is one launch: rows go from the projection's output straight to their pages
-// (8892 tokens of 32 + 8 + 8 heads of 128 in bf16: 43.2 us, 5.1 TB/s).
+// (8892 tokens of 32 + 8 + 8 heads of 128 in bf16: 41.8 us, 5.2 TB/s).
 #include "paged_common.cuh"
 #include <algorithm>
 #include <cmath>
@@ -235,9 +235,9 @@ int launch_t(b200_ctx *ctx, const RopeArgs &r, const PagedArgs &a, bool vec) {
   const dim3 grid((unsigned)((r.tokens + r.per_cta - 1) / r.per_cta));
   const unsigned long long most = (unsigned long long)r.tokens * std::max(std::max(r.ld_q, r.ld_qo), std::max(r.ld_k, r.ld_ko));
   const bool small = (unsigned long long)(r.ld_q | r.ld_qo | r.ld_k | r.ld_ko) < (1ull << 31) && most < (1ull << 32);
-  if (vec && small) B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, true, unsigned>, grid, dim3(THREADS), 0, 0, r, a));
-  else if (vec) B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, true, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
-  else B200_CUDA(ctx, launch_k(ctx, rope_positions_kernel<T, HALF, false, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
+  if (vec && small) B200_CUDA(ctx, launch_pdl(ctx, rope_positions_kernel<T, HALF, true, unsigned>, grid, dim3(THREADS), 0, 0, r, a));
+  else if (vec) B200_CUDA(ctx, launch_pdl(ctx, rope_positions_kernel<T, HALF, true, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
+  else B200_CUDA(ctx, launch_pdl(ctx, rope_positions_kernel<T, HALF, false, unsigned long long>, grid, dim3(THREADS), 0, 0, r, a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
@@ -303,7 +303,7 @@ extern "C" int b200_rope_frequencies(b200_ctx *ctx, const b200_rope_config *c, d
   DeviceGuard guard(ctx);
   B200_REQUIRE(ctx, guard.ok, "rope_frequencies: the context's device cannot be selected");
   const int pairs = (int)(c->rotary_dim / 2);
-  B200_CUDA(ctx, launch_k(ctx, rope_frequencies_kernel, dim3((pairs + 127) / 128), dim3(128), 0, 0, freqs, pairs, *c));
+  B200_CUDA(ctx, launch_pdl(ctx, rope_frequencies_kernel, dim3((pairs + 127) / 128), dim3(128), 0, 0, freqs, pairs, *c));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }

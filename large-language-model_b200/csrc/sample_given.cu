@@ -16,8 +16,8 @@
 //   * The ids of a border's bin are ranked against each other; a bin with more ids than the list holds is cut again by the bits of
 //     its values, at most three times; equal values are settled by arithmetic.
 // The kept set is a prefix of the order: a least value and the number of ids of that value, lowest ids first.
-// Bound by latency at usual sizes (64 rows of 32000 ids in bf16 with all filters: 16.4 us, five exchanges within the cluster) and by instructions, the
-// 64-bit exponentials above all, for large vocabularies (32 rows of 100256 ids in 32 bits, nucleus alone: 39.7 us); the floor is one read of
+// Bound by latency at usual sizes (64 rows of 32000 ids in bf16 with all filters: 13.9 us, five exchanges within the cluster) and by instructions, the
+// 64-bit exponentials above all, for large vocabularies (32 rows of 100256 ids in 32 bits, nucleus alone: 38 us); the floor is one read of
 // the logits (0.6 and 2 us).
 #include "paged_common.cuh"
 #include <algorithm>
@@ -733,7 +733,7 @@ int launch_t(b200_ctx *ctx, const GivenArgs &a, size_t batch, size_t smem) {
   static std::atomic<unsigned long long> attr{0};
   const unsigned long long bit = 1ull << (ctx->device & 63);
   if (!(attr.load() & bit)) { B200_CUDA(ctx, cudaFuncSetAttribute(sample_given_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024)); attr.fetch_or(bit); }
-  B200_CUDA(ctx, launch_k(ctx, sample_given_kernel<T, C>, dim3((unsigned)(batch * C)), dim3(THREADS), smem, C > 1 ? C : 0, a));
+  B200_CUDA(ctx, launch_pdl(ctx, sample_given_kernel<T, C>, dim3((unsigned)(batch * C)), dim3(THREADS), smem, C > 1 ? C : 0, a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
