@@ -191,65 +191,70 @@ paged_attn_simt_kernel(PagedAttnArgs a) {
 }
 
 // ---- join: one CTA column per border between runs; it works when the border is the first one inside its block ------------
-// A thread owns four dimensions of a row and adds its parts in CTA order, the loads of four parts in flight at once (chains of
-// dependent loads made this kernel 40 to 70 us long).  With more than eight parts the CTA's eight warps share them out and add their sums.
+// A thread owns D dimensions of a row (eight where the head and the alignment allow: the maxima and weights of a row's parts are then looked at half as
+// often; with four this kernel was bound by instructions, 23 us of a 127 us mixed batch) and adds its parts in CTA order, two parts in flight at
+// once.  With more than eight parts the CTA's eight warps share them out and add their sums.
 constexpr int JOIN_THREADS = 256, JOIN_WARPS = JOIN_THREADS / 32;
-template <class T>
+template <class T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_join_kernel(PagedAttnArgs a, PagedAttnArgs a2) {
   pdl_wait();
   pdl_launch_dependents();
   int c = blockIdx.x + 1;
-  if (c >= a.n_cta) { c -= a.n_cta - 1; a = a2; }      // the second kernel's borders follow the first's
-  __shared__ float sh_m[JOIN_WARPS][32], sh_l[JOIN_WARPS][32];
-  __shared__ float4 sh_e[JOIN_WARPS][32];
-  const int hd = a.b.hd, tid = threadIdx.x;
-  const JoinHead *head_ = paged_head(a, c);
+  const bool second = c >= a.n_cta;                    // the second kernel's borders follow the first's
+  const PagedAttnArgs &p = second ? a2 : a;
+  if (second) c -= a.n_cta - 1;
+  __shared__ float sh_m[JOIN_WARPS][32], sh_l[JOIN_WARPS][32], sh_e[JOIN_WARPS][D][32];
+  const int hd = p.b.hd, tid = threadIdx.x;
+  const JoinHead *head_ = paged_head(p, c);
   const int parts = head_->parts;
   if (parts == 0) return;
   const paged::Place pl = head_->pl;
-  const float *part0 = paged_slot(a, c - 1, true), *part1 = paged_slot(a, c, false);
-  const size_t step = 2 * paged_slot_floats(a.slot_rows, hd);
-  const int vecs = (hd + 3) / 4, items = a.slot_rows * vecs, groups = parts > 8 ? JOIN_WARPS : 1, width = JOIN_THREADS / groups;
-  const int group = tid / width, k0 = (int)((long long)parts * group / groups), k1 = (int)((long long)parts * (group + 1) / groups);
+  const float *part0 = paged_slot(p, c - 1, true), *part1 = paged_slot(p, c, false);
+  const size_t step = 2 * paged_slot_floats(p.slot_rows, hd);
+  const int vecs = (hd + D - 1) / D, items = p.slot_rows * vecs, groups = parts > 8 ? JOIN_WARPS : 1, width = JOIN_THREADS / groups;
+  const int group = groups > 1 ? tid >> 5 : 0, k0 = parts * group / groups, k1 = parts * (group + 1) / groups;
   for (int i0 = blockIdx.y * width; i0 < items; i0 += gridDim.y * width) {
-    const int i = i0 + tid % width;
-    const int r = i / vecs, d = (i - r * vecs) * 4;
+    const int i = i0 + (tid & (width - 1)), r = i / vecs, d = (i - r * vecs) * D;
     const size_t at = (size_t)r * hd + d;
     int row = 0, head = 0, pos = 0;
-    const bool has = i < items && paged_row(a, pl, r, row, head, pos);
-    const bool vec = hd % 4 == 0;
-    float mx = -INFINITY, l = 0.f, e[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool has = i < items && paged_row(p, pl, r, row, head, pos);
+    float mx = -INFINITY, l = 0.f, e[D];
+#pragma unroll
+    for (int x = 0; x < D; ++x) e[x] = 0.f;
     if (has) {
-      const size_t at_m = (size_t)a.slot_rows * hd + r, at_l = at_m + a.slot_rows;
-      for (int k = k0; k < k1; k += 4) {
-        float m4[4], l4[4], e4[4][4], top = mx;
+      const size_t at_m = (size_t)p.slot_rows * hd + r, at_l = at_m + p.slot_rows;
+      for (int k = k0; k < k1; k += 2) {
+        float m2[2], l2[2], e2[2][D];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float *p = k + j == 0 ? part0 : part1 + (size_t)(k + j - 1) * step;
-          const bool in = k + j < k1;
-          m4[j] = in ? p[at_m] : -INFINITY;
-          l4[j] = in ? p[at_l] : 0.f;
-          if (vec) { const float4 x = in ? *reinterpret_cast<const float4 *>(p + at) : make_float4(0.f, 0.f, 0.f, 0.f); e4[j][0] = x.x; e4[j][1] = x.y; e4[j][2] = x.z; e4[j][3] = x.w; }
-          else {
+        for (int j = 0; j < 2; ++j) {
+          const float *q = k + j == 0 ? part0 : part1 + (size_t)(k + j - 1) * step;
+          m2[j] = -INFINITY; l2[j] = 0.f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) e4[j][x] = in && d + x < hd ? p[at + x] : 0.f;
+          for (int x = 0; x < D; ++x) e2[j][x] = 0.f;
+          if (k + j < k1) {
+            m2[j] = q[at_m]; l2[j] = q[at_l];
+            if constexpr (D == 8) {
+              const float4 u = *reinterpret_cast<const float4 *>(q + at), v = *reinterpret_cast<const float4 *>(q + at + 4);
+              e2[j][0] = u.x; e2[j][1] = u.y; e2[j][2] = u.z; e2[j][3] = u.w; e2[j][4] = v.x; e2[j][5] = v.y; e2[j][6] = v.z; e2[j][7] = v.w;
+            } else {
+#pragma unroll
+              for (int x = 0; x < D; ++x) if (d + x < hd) e2[j][x] = q[at + x];
+            }
           }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, m4[j]);
-        const float base = top == -INFINITY ? 0.f : top, f = exp2f(mx - base);
+        const float top = fmaxf(mx, fmaxf(m2[0], m2[1])), base = top == -INFINITY ? 0.f : top, f = exp2f(mx - base);
+        mx = top;
         l *= f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) e[x] *= f;
-        mx = top;
+        for (int x = 0; x < D; ++x) e[x] *= f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float wt = exp2f(m4[j] - base);
+        for (int j = 0; j < 2; ++j) {
+          const float wt = exp2f(m2[j] - base);
           if (wt > 0.f) {                                    // a part that saw no key holds anything
-            l = fmaf(wt, l4[j], l);
+            l = fmaf(wt, l2[j], l);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) e[x] = fmaf(wt, e4[j][x], e[x]);
+            for (int x = 0; x < D; ++x) e[x] = fmaf(wt, e2[j][x], e[x]);
           }
         }
       }
@@ -257,31 +262,37 @@ paged_join_kernel(PagedAttnArgs a, PagedAttnArgs a2) {
     if (groups > 1) {
       const int lane = tid & 31;
       __syncthreads();
-      sh_m[group][lane] = mx; sh_l[group][lane] = l; sh_e[group][lane] = make_float4(e[0], e[1], e[2], e[3]);
+      sh_m[group][lane] = mx; sh_l[group][lane] = l;
+#pragma unroll
+      for (int x = 0; x < D; ++x) sh_e[group][x][lane] = e[x];
       __syncthreads();
       if (group == 0) {
         for (int k = 0; k < JOIN_WARPS; ++k) mx = fmaxf(mx, sh_m[k][lane]);
         const float base = mx == -INFINITY ? 0.f : mx;
-        l = e[0] = e[1] = e[2] = e[3] = 0.f;
+        l = 0.f;
+#pragma unroll
+        for (int x = 0; x < D; ++x) e[x] = 0.f;
         for (int k = 0; k < JOIN_WARPS; ++k) {
           const float wt = exp2f(sh_m[k][lane] - base);
-          const float4 x = sh_e[k][lane];
           l = fmaf(wt, sh_l[k][lane], l);
-          e[0] = fmaf(wt, x.x, e[0]); e[1] = fmaf(wt, x.y, e[1]); e[2] = fmaf(wt, x.z, e[2]); e[3] = fmaf(wt, x.w, e[3]);
+#pragma unroll
+          for (int x = 0; x < D; ++x) e[x] = fmaf(wt, sh_e[k][x][lane], e[x]);
         }
       }
     }
     if (has && group == 0) {
       const float inv = l > 0.f ? 1.0f / l : 0.f;
-      T *dst = (T *)a.o + (size_t)row * a.ld_o + (size_t)head * hd + d;
-      if (a.vec_out && sizeof(T) == 2) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0] * inv, e[1] * inv), hi = __floats2bfloat162_rn(e[2] * inv, e[3] * inv);
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+      T *dst = (T *)p.o + (size_t)row * p.ld_o + (size_t)head * hd + d;
+      if constexpr (D == 8 && sizeof(T) == 2) {
+        uint32_t w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) { const __nv_bfloat162 h = __floats2bfloat162_rn(e[2 * x] * inv, e[2 * x + 1] * inv); w[x] = *reinterpret_cast<const uint32_t *>(&h); }
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) if (d + x < hd) dst[x] = from_f<T>(e[x] * inv);
+        for (int x = 0; x < D; ++x) if (d + x < hd) dst[x] = from_f<T>(e[x] * inv);
       }
-      if (a.lse && d == 0) a.lse[(size_t)row * a.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
+      if (p.lse && d == 0) p.lse[(size_t)row * p.nH + head] = l > 0.f ? (mx + log2f(l)) / PAGED_LOG2E : -INFINITY;
     }
   }
 }
@@ -311,9 +322,11 @@ constexpr int MIN_UNITS = 1;
 int paged_join_launch(b200_ctx *ctx, const PagedAttnArgs &a, const PagedAttnArgs *b, b200_dtype dt) {
   const int borders = a.n_cta - 1 + (b ? b->n_cta - 1 : 0), rows = std::max(a.slot_rows, b ? b->slot_rows : 0);
   if (borders < 1) return B200_OK;
-  const dim3 grid((unsigned)borders, (unsigned)std::min(16, (rows * ((a.b.hd + 3) / 4) + JOIN_THREADS - 1) / JOIN_THREADS));
-  if (dt == B200_BF16) B200_CUDA(ctx, launch_pdl(ctx, paged_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a));
-  else B200_CUDA(ctx, launch_pdl(ctx, paged_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a));
+  const bool eight = a.vec_out && a.b.hd % 8 == 0;      // both kernels of a call have the same head and alignment
+  const dim3 grid((unsigned)borders, (unsigned)std::min(16, (rows * (a.b.hd / (eight ? 8 : 4) + (eight ? 0 : 1)) + JOIN_THREADS - 1) / JOIN_THREADS));
+  if (dt == B200_F32) B200_CUDA(ctx, launch_pdl(ctx, paged_join_kernel<float, 4>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a));
+  else if (eight) B200_CUDA(ctx, launch_pdl(ctx, paged_join_kernel<bf16, 8>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a));
+  else B200_CUDA(ctx, launch_pdl(ctx, paged_join_kernel<bf16, 4>, grid, dim3(JOIN_THREADS), 0, 0, a, b ? *b : a));
   B200_LAUNCHED(ctx);
   return B200_OK;
 }
@@ -364,7 +377,7 @@ extern "C" int b200_paged_attn(b200_ctx *ctx, const b200_paged_cache *cache, con
   if (many) {
     if (tc) rc = paged_attn_tc_launch(ctx, a, G, few ? PAGED_FEW_ROWS + 1 : 0);
     else {
-      a.vec_out = 0; a.beside = 0;
+      a.vec_out = fast; a.beside = 0;                   // (`fast` implies aligned output rows)
       a.plan = paged::Plan{G, 0, ROWS, 5, 1, few ? PAGED_FEW_ROWS + 1 : 0, 0x7fffffff};
       a.n_cta = 2 * ctx->sm_count; a.min_units = MIN_UNITS; a.slot_rows = ROWS;
       rc = cache->dtype == B200_BF16 ? simt_launch<bf16>(ctx, a) : simt_launch<float>(ctx, a);

@@ -105,3 +105,9 @@ def test_large_vocabulary_beyond_shared_memory(ctx):
     x = np.random.RandomState(2).randn(B, V).astype(np.float32) * 3
     for kw in (dict(), dict(k=50), dict(p=0.9, T=0.7)):
         check(ctx, x, np.array([0.2, 0.9], np.float32), **kw)
+
+
+def test_the_largest_vocabulary(ctx):
+    x = np.random.RandomState(4).randn(1, 1 << 24).astype(np.float32) * 2
+    for kw in (dict(k=50, p=0.9), dict(p=0.5), dict(k=1 << 20, m=1e-4)):
+        check(ctx, x, np.array([0.7], np.float32), dtype="bf16", **kw)
