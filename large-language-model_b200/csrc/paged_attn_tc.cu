@@ -13,7 +13,7 @@
 //     partial result for the join.
 // A block with rows for one tile only leaves the other idle; giving both alternate key tiles of the same rows was no faster (two buffers
 // of keys and of values then hold no tile ahead: 3.2 thousand cycles a key tile against 4.2, and 6 thousand more to join the two; mixed batch 150 us
-// against 127).
+// against 127 then, 119 now).
 // 1024 tokens over 30011 positions, 32 query and 8 KV heads of 128: 485 us by itself (1.02 PFLOP/s), 600 us in a loop of its own at the power limit
 // (0.82 PFLOP/s, half the matrix rate).  A key tile takes 2.3 to 2.5 us for 256 rows in long runs; a block's start and end about 10 us, which
 // is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us, before the last two steps): the boxes of
@@ -28,16 +28,17 @@ using namespace attn;
 
 namespace {
 
+constexpr int TC_THREADS = 384, TC_WARPS = TC_THREADS / 32, FIX_WARP = 10;
 struct alignas(16) TcShared {
   uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], fix_ask[2], fix_done[2], s_full[2], p_full[2], o_full[2];
   uint32_t tmem_base;
   int abort_flag;
   long long red[33];
   paged::Place place;
+  paged::Walk walk[TC_WARPS];      // each warp's own, to save registers (with 208 for the softmax warps and the walk in them, spills in the tile loop cost 20 %)
 };
 
 constexpr float RESCALE_THRESHOLD = 8.0f;      // log2 units: P stays below 2^8
-constexpr int TC_THREADS = 384, FIX_WARP = 10;
 constexpr int REGS_SOFTMAX = 216, REGS_SERVICE = 72;      // 8 x 32 x 216 + 4 x 32 x 72 = 384 x 168, the launch's share
 template <int N> __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -107,9 +108,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   tc::tc_fence_after();
   const uint32_t tmem_base = sh->tmem_base;
   const long long end = run.end;
-  paged::Walk w;
-  w.start(a.plan, sh->place, end);
-  paged::Place &pl = w.pl;
+  paged::Walk &w = sh->walk[warp];
+  if (lane == 0) w.start(a.plan, sh->place, end);
+  __syncwarp();
+  const paged::Place &pl = w.pl;
+  auto next = [&] { __syncwarp(); if (lane == 0) w.next(a.b, a.plan, end); __syncwarp(); };
   int seg = 0;                                   // segments so far
   bool ok = true;
 
@@ -168,7 +171,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (lane == 0 && j == ragged) tc::mbar_arrive(&sh->fix_ask[s]);
           page = next;
         }
-        w.next(a.b, a.plan, end);
+        next();
       }
       if (*abort_flag) { long long t0 = clock64(); while (clock64() - t0 < 2000000ll) {} }      // copies in flight land before the CTA ends
     } else if (warp == MMA_WARP) {
@@ -250,7 +253,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (lane == 0) tc::mbar_arrive(&sh->fix_done[s]);
         }
         it += g.k1 - g.k0;
-        w.next(a.b, a.plan, end);
+        next();
       }
     }
   } else {
@@ -399,7 +402,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         } else if (a.lse) a.lse[(long long)row * a.nH + head] = l > 0.f ? (m_used + log2f(l)) / PAGED_LOG2E : -INFINITY;
       }
       tc::tc_fence_before();
-      w.next(a.b, a.plan, end);
+      next();
     }
   }
   tc::tc_fence_before();
