@@ -202,7 +202,7 @@ int b200_flash_attn_bwd(b200_ctx *ctx, const void *Q, const void *K, const void 
  * Sequences may share pages (a common prefix).  The tables and lengths are read on the device, so a captured step replays with
  * new ones.  What they say is checked there: a page id outside [0, n_pages), a length beyond the table, or rows that q_start
  * puts outside [0, rows) touch no memory outside the arrays; b200_sync then reports B200_ERR_INVALID, and the results of
- * that sequence are unspecified. */
+ * that batch are unspecified. */
 typedef struct {
   void *k, *v;                                             /* device */
   size_t n_pages, page_size, n_kv, head_dim;
@@ -224,7 +224,7 @@ int b200_paged_append(b200_ctx *ctx, const b200_paged_cache *cache, const b200_p
                       size_t ld_v, const b200_rope_config *rope, const double *freqs, const void *q, void *q_out, size_t ld_q,
                       size_t ld_q_out, size_t q_heads);
 /* Causal attention of the new rows over the cache (which holds them already): o [rows, n_heads, head_dim] and, optional, lse fp32
- * [rows, n_heads], the log-sum-exp of the scaled scores.  scale 0: 1/sqrt(head_dim).  Rows that see nothing get o = 0, lse = -inf.
+ * [rows, n_heads], the log-sum-exp (natural) of the scaled scores.  scale 0: 1/sqrt(head_dim).  Rows that see nothing get o = 0, lse = -inf.
  * Positions from kv_len on are never used, whatever their slots hold; values inside must be finite.  head_dim up to 256.  o must not
  * overlap q.  Fast paths: bf16, head_dim 64 or 128, 16-byte aligned rows, for chunks also a page_size that is a multiple of 8 and at most 128
  * query heads per KV head; everything else runs on CUDA cores.
