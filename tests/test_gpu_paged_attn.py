@@ -204,6 +204,9 @@ def test_arrays_of_the_wrong_kind_are_refused(ctx):
         kw = {**dict(q=m.d_q, out=m.out, lse=m.lse), **bad}
         with pytest.raises(bridge.B200Error):
             ctx.paged_attn(m.cache, m.batch, **kw)
+    need = ctx.paged_attn_workspace(m.cache, m.batch, 4)
+    with pytest.raises(bridge.B200Error, match="workspace"):
+        ctx.paged_attn(m.cache, m.batch, m.d_q, out=m.out, workspace=ctx.empty((need // 4 - 1,)))
     with pytest.raises(bridge.B200Error):
         ctx.rope_positions_forward(bridge.RopeConfig.make(64), ctx.empty((32,), "f32"), ctx.empty((3,), "i32"), m.d_q)
     with pytest.raises(bridge.B200Error):

@@ -53,7 +53,7 @@ def test_bad_batches(lib, ctx, kw):
     assert lib.b200_paged_append(ctx, C.byref(cache()), C.byref(batch(**kw)), P, P, 128, 128, None, None, None, None, 0, 0, 0) == INVALID
 
 
-@pytest.mark.parametrize("kw", [dict(q=None), dict(o=None), dict(ld_q=511), dict(ld_o=511), dict(nH=0), dict(nH=7), dict(scale=float("nan")), dict(scale=-1.0), dict(ws=None), dict(n=100), dict(ws=P + 4)])
+@pytest.mark.parametrize("kw", [dict(q=None), dict(o=None), dict(ld_q=511), dict(ld_o=511), dict(nH=0), dict(nH=7), dict(scale=float("nan")), dict(scale=-1.0), dict(ws=None), dict(ws=P + 4)])
 def test_bad_attention_calls(lib, ctx, kw):
     assert attn(lib, ctx, **kw) == INVALID
 
