@@ -14,9 +14,9 @@
 // A block with rows for one tile only leaves the other idle; giving both alternate key tiles of the same rows was no faster (two buffers
 // of keys and of values then hold no tile ahead: 3.2 thousand cycles a key tile against 4.2, and 6 thousand more to join the two; mixed batch 150 us
 // against 127 then, 119 now).
-// 1024 tokens over 30011 positions, 32 query and 8 KV heads of 128: 485 us by itself (1.02 PFLOP/s), 600 us in a loop of its own at the power limit
-// (0.82 PFLOP/s, half the matrix rate).  A key tile takes 2.3 to 2.5 us for 256 rows in long runs; a block's start and end about 10 us, which
-// is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us, before the last two steps): the boxes of
+// 1024 tokens over 30011 positions, 32 query and 8 KV heads of 128: 490 us by itself (1.01 PFLOP/s), 600 us in a loop of its own at the power limit
+// (0.82 PFLOP/s, half the matrix rate).  A key tile takes 2.3 to 2.5 us for 256 rows in long runs; a block's start and end about 5 us (a CTA's
+// first 7), which is what bounds batches of short chunks.  Asking the L2 cache for tiles two ahead made it slower (mixed batch 149 -> 190 us, before the last two steps): the boxes of
 // small pages already fill the copy engine's issue rate.
 // Tensor memory: [S_A 128 | O_A 128 | S_B 128 | O_B 128] columns.  Warps 0-3 softmax of tile A, 4-7 of tile B, 8 MMA issue, 9 loads, 10 value rows.
 #include "attention_tc.cuh"

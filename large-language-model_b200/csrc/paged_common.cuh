@@ -80,7 +80,7 @@ __host__ __device__ __forceinline__ int page_of(const PagedArgs &a, int s, int p
 // ---- division of the work ---------------------------------------------------------------------------------------------
 // A sequence's rows (token, query head of the group) are cut into blocks; a block walks the key tiles its last row can see.
 // All (sequence, KV head, block, tile) in this order form one line; a block takes `extra` units (its start and end, in tiles' time)
-// and one per tile.  CTA c of n works on units [c * total / n, (c + 1) * total / n): every SM gets the same amount of work
+// and one per tile.  The line is cut into n runs of equal length (the first total % n have one unit more): every SM gets the same amount of work
 // whatever the lengths are (without the extra, CTAs whose run held dozens of short sequences took 1.8 times the others' time).
 // A block that crosses a border leaves partial results (unnormalised output, maximum, sum) that a second kernel joins in CTA order.
 struct Plan {
